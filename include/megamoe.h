@@ -24,6 +24,9 @@
  *   mm_layer_create      RoutedExpertGemm.__init__, routed_expert_gemm.py:537-657
  *   mm_layer_experts     RoutedExpertGemm.__call__, routed_expert_gemm.py:703-774
  *   mm_layer_gate_experts RoutedExpertGemm.gate_topk_and_gemms, routed_expert_gemm.py:776-870
+ *   mm_rms_norm          deepseek_v41/sm103/all_reduce_mhc.py:665-1190 (the RMSNorm and
+ *                        MXFP8 epilogue, without the exchange)
+ *   mm_int8_ffn          the place of deepseek_v41/moe/shared_ll.py:1-20, at int8
  *   mm_finalize          deepseek_v41/sm103/all_reduce_mhc.py:402-662 (finalize arithmetic);
  *                        glm5_3/sm103/moe/finalize.py:1-27
  *   mm_layer_forward     deepseek_v41/moe/step.py:101 (one MoE step: router -> combine)
@@ -208,6 +211,51 @@ typedef struct mm_forward_args {
   uint16_t *residual_out;   /* bf16 [T, H] new residual (may alias residual)   */
 } mm_forward_args;
 
+/* ---- dense 8-bit operators ------------------------------------------------ */
+/* Element types of activations and outputs. */
+#define MM_DTYPE_BF16 0
+#define MM_DTYPE_FP16 1
+#define MM_DTYPE_FP32 2
+
+/* 8-bit outputs of mm_rms_norm. */
+#define MM_QUANT_NONE 0
+#define MM_QUANT_MXFP8 1 /* E4M3 codes, an E8M0 scale per 32 values: 2^e, e = ceil(log2(amax / 448)),
+                            scale 1 for a zero block; a block with a value that is not finite gets
+                            scale code 255 (NaN). The routed input of mm_layer_experts_mxfp8.     */
+#define MM_QUANT_INT8 2  /* int8 codes in -127..127, an fp32 scale per row: s = amax / 127, codes
+                            rint(y / s); s = 0 for a zero row; s = NaN and codes 0 for a row with
+                            a value that is not finite. The input of mm_int8_linear.              */
+
+typedef struct mm_norm_args {
+  const void *x;          /* [tokens, hidden] of dtype, rows ld_x elements apart             */
+  const void *residual;   /* the same (rows ld_residual apart), or NULL                      */
+  const void *gamma;      /* [hidden] of dtype or fp32 (gamma_dtype)                         */
+  void *residual_out;     /* with residual: x + residual; may be residual or x itself        */
+  void *norm_out;         /* the norm in dtype, or NULL (then quant is not NONE)             */
+  void *codes;            /* u8 / int8 [tokens, hidden], rows ld_codes bytes apart           */
+  void *scales;           /* E8M0 u8 [tokens, hidden / 32] or fp32 [tokens]                  */
+  int64_t ld_x, ld_residual, ld_residual_out, ld_norm, ld_codes;
+  int32_t tokens, hidden; /* hidden: any >= 1; MXFP8: a multiple of 32                       */
+  int32_t dtype, gamma_dtype, quant;
+  float eps;
+} mm_norm_args;
+
+typedef struct mm_int8_ffn_args {
+  const int8_t *x;         /* [tokens, hidden] codes, rows ld_x bytes apart                   */
+  const float *x_scale;    /* [tokens]                                                        */
+  const int8_t *w13;       /* [2 * inter, hidden], rows ld_w13 apart: [0, inter) gate, then up */
+  const float *w13_scale;  /* [2 * inter]                                                     */
+  const int8_t *w2;        /* [hidden, inter], rows ld_w2 apart                               */
+  const float *w2_scale;   /* [hidden]                                                        */
+  void *out;               /* [tokens, hidden] of out_dtype, rows ld_out elements apart       */
+  void *workspace;         /* mm_int8_ffn_workspace bytes on a 256-byte boundary; calls that
+                              may run at the same time need one each                          */
+  int64_t workspace_bytes;
+  int64_t ld_x, ld_w13, ld_w2, ld_out;
+  int32_t tokens, hidden, inter, out_dtype;
+  float clamp;             /* > 0: gate <= clamp, -clamp <= up <= clamp; 0: none              */
+} mm_int8_ffn_args;
+
 /* ---- library ------------------------------------------------------------ */
 const char *mm_last_error(void);
 int mm_version(void);
@@ -262,6 +310,40 @@ int mm_finalize(const uint16_t *rows, const float *weights, const int32_t *permu
 /* out = bf16(bf16(sum_r routed_r) + sum_r shared_r) from an all-reduced partial. */
 int mm_finalize_partial(const float *partial, uint16_t *out, int32_t tokens,
                         int32_t hidden, void *stream);
+
+/* The residual's addition, the RMSNorm and its 8-bit output in one launch, per row:
+ *   r = round(x + residual), residual_out = r   (r = x without a residual)
+ *   y = (r * (1 / sqrt(sum(r^2) / hidden + eps))) * gamma   (fp32)
+ *   norm_out = round(y); codes and scales of y (not of the rounded norm)
+ * What the reference's hop fuses behind its all-reduce (deepseek_v41/sm103/
+ * all_reduce_mhc.py:665-1190: RMSNorm and the MXFP8 of the next input), for one
+ * GPU's rows. Like every call below: on the current device, which holds the
+ * buffers; 0 tokens launch nothing. */
+int mm_rms_norm(const mm_norm_args *args, void *stream);
+
+/* int8 codes and scales (MM_QUANT_INT8) of rows as they are. */
+int mm_quantize_int8(const void *x, int64_t ld_x, int32_t dtype, int8_t *codes, int64_t ld_codes,
+                     float *scales, int32_t tokens, int32_t hidden, void *stream);
+
+/* out[t, n] = round((sum_k x[t, k] w[n, k]) * x_scale[t] * w_scale[n] + bias[n]):
+ * int8 codes with a scale per token and per channel, the sum an exact 32-bit integer.
+ * x and w rows start on 16-byte boundaries (base and row stride); bias fp32 or NULL.
+ * depth < 131072. */
+int mm_int8_linear(const int8_t *x, int64_t ld_x, const float *x_scale, const int8_t *w, int64_t ld_w,
+                   const float *w_scale, const float *bias, void *out, int64_t ld_out,
+                   int32_t out_dtype, int32_t tokens, int32_t features, int32_t depth, void *stream);
+
+/* The gated feed-forward block over int8 weights: h = silu(gate) * up of the products
+ * with w13 (clamped first), in fp32; its int8 codes and scales by row; out = their
+ * product with w2. A model's dense layers, and the shared expert at 8 bits (the
+ * reference's shared expert, deepseek_v41/moe/shared_ll.py:1-20, is MXFP8): out is
+ * then mm_finalize's shared_rows. */
+int64_t mm_int8_ffn_workspace(int32_t tokens, int32_t inter);
+int mm_int8_ffn(const mm_int8_ffn_args *args, void *stream);
+
+/* Synchronizes the current device and reads (then clears) the error word of the int8
+ * products' bounded waits on it: MM_OK or MM_ERR_DEVICE_TIMEOUT. */
+int mm_int8_check(void);
 
 /* ---- combine + all-reduce over NVLink peer memory ------------------------ */
 /* One rank's view of a TP/EP group whose ranks exchange their partial outputs

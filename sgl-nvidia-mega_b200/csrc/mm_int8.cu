@@ -1,0 +1,510 @@
+// Products in 8-bit integers with a scale for each token and each channel, and the gated
+// feed-forward block made of two of them:
+//   out[t, n] = round( ((float) sum_k x[t, k] w[n, k]) * xs[t] * ws[n] + bias[n] )
+//   h[t, i]   = silu(gate) * up  of the products with rows i and I + i of w13, in fp32
+// The sums are exact 32-bit integers (at most 2^17 - 1 products of at most 2^14), so they do
+// not depend on how the depth is split or in which order the parts are added; what follows is
+// fp32 and one rounding to the output's type.
+//
+// tcgen05 kind::i8, operands by TMA as 128-byte-swizzled K-major boxes of 128 bytes of depth.
+// Two forms:
+//  * int8_stream_kernel (few tokens; bound by the weights' stream). 128 weight rows are the
+//    MMA's M side and up to 256 tokens its N side, so one token costs one column and the
+//    tokens' padding costs no memory traffic. Few tiles do not fill the GPU: the CTAs of a
+//    cluster share a tile's depth, and add their integer parts through distributed shared
+//    memory, each finishing its share of the tokens. No workspace, no atomics, no counters.
+//  * int8_tile_kernel (many tokens; bound by the tensor pipe). A CTA pair owns 256 tokens x
+//    256 weight rows (cta_group::2: each CTA stages half of either operand, half the shared
+//    memory traffic of two single tiles), persistent, with two accumulators in TMEM so that
+//    the epilogue of one tile runs under the products of the next.
+// A gated tile takes 128 gate rows and the 128 up rows of the same features into two halves
+// of the accumulator: gate and up of one element sit in the same TMEM lane.
+#include <algorithm>
+#include <cstdint>
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include "megamoe.h"
+#include "mm_dense.cuh"
+#include "mm_kernels.cuh"
+#include "mm_ptx.cuh"
+
+namespace mm {
+namespace {
+
+constexpr int kBlockK = 128;          // depth of a stage, bytes
+constexpr int kRowsM = 128;           // weight rows of a box, token rows of a pair's half
+constexpr int kBoxBytes = kRowsM * kBlockK;
+
+// Error word of this file's launches: bounded waits that ran out (mm_int8_check).
+__device__ uint32_t g_int8_error;
+
+struct alignas(64) Int8Args {
+  CUtensorMap w_map;    // {depth, rows, planes}: plane 1 holds the up rows of w13
+  CUtensorMap x_map;    // {depth, tokens}
+  CUtensorMap out_map;  // {features, tokens}, where stage_out
+  const float *x_scale, *w_scale, *bias;
+  void *out;
+  int64_t ld_out;
+  int tokens, features, blocks_k;
+  int out_type;
+  int stage_out;        // output rows start on 16-byte boundaries: TMA stores
+  int gated;
+  int has_clamp;
+  float clamp;
+  int token_tiles, feature_tiles;  // of the tile form
+  int split;            // CTAs of a cluster that share a tile's depth (stream form)
+};
+
+__device__ __forceinline__ float gate_up(const Int8Args &p, float g, float u) {
+  if (p.has_clamp) {
+    // NaN stays NaN: comparisons instead of fminf / fmaxf
+    g = g > p.clamp ? p.clamp : g;
+    u = u > p.clamp ? p.clamp : u;
+    u = u < -p.clamp ? -p.clamp : u;
+  }
+  return __fmul_rn(u, __fdiv_rn(g, __fadd_rn(1.0f, expf(-g))));
+}
+
+// Four consecutive features of one token.
+__device__ __forceinline__ void store4(const Int8Args &p, int64_t at, int left, const float (&v)[4], bool wide) {
+  if (p.out_type == MM_DTYPE_FP32) {
+    float *o = static_cast<float *>(p.out) + at;
+    if (wide && left >= 4) {
+      *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < left) o[i] = v[i];
+    }
+  } else {
+    uint16_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      h[i] = p.out_type == MM_DTYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v[i]))
+                                         : __half_as_ushort(__float2half_rn(v[i]));
+    uint16_t *o = static_cast<uint16_t *>(p.out) + at;
+    if (wide && left >= 4) {
+      *reinterpret_cast<uint2 *>(o) = make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < left) o[i] = h[i];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// The stream form. Two CTAs share an SM (at most 113 KB each), so that one's start, its
+// accumulator read and its reduction run under the other's loads.
+template <int BN, bool GATED>
+struct Stream {
+  static constexpr int kA = GATED ? 2 : 1;
+  static constexpr int kStageBytes = kA * kBoxBytes + BN * kBlockK;
+  static constexpr int kRing = 108 * 1024;
+  static constexpr int kStages = kRing / kStageBytes;
+  // tokens whose parts are staged at once: 64 KB at most, in the ring's place
+  static constexpr int kChunk = BN < 128 / kA ? BN : 128 / kA;
+  static constexpr int kCols = kA * BN < 32 ? 32 : kA * BN;  // TMEM columns, a power of two
+  static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+  static_assert(kStages >= 2 && kCols <= 256, "two CTAs an SM share 512 columns");
+  static_assert(kChunk * kA * 512 <= kStages * kStageBytes, "parts fit the ring");
+};
+
+constexpr int kStreamThreads = 192;
+constexpr int kStreamWarps = kStreamThreads / 32;
+
+template <int BN, bool GATED>
+__global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __grid_constant__ Int8Args p) {
+  using S = Stream<BN, GATED>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t ring = (raw + 1023u) & ~1023u;
+  uint8_t *ring_ptr = smem_raw + (ring - raw);
+  const uint32_t bars = ring + S::kStages * S::kStageBytes;
+  const uint32_t full = bars, empty = bars + 8 * S::kStages, acc = bars + 16 * S::kStages, slot = acc + 8;
+  uint32_t *slot_ptr = reinterpret_cast<uint32_t *>(ring_ptr + (slot - ring));
+  volatile uint32_t *failed = slot_ptr + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = p.split;
+  const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int f0 = (blockIdx.x / split) * kRowsM;
+  const int t0 = blockIdx.y * BN;
+  const int kb0 = p.blocks_k * rank / split, kb1 = p.blocks_k * (rank + 1) / split;
+  const int n = kb1 - kb0;
+
+  if (warp == 0 && lane == 0) {
+    // the weights do not depend on the launch before this one: bring the first stages into L2
+    tma_prefetch_desc(&p.w_map);
+    tma_prefetch_desc(&p.x_map);
+#pragma unroll 1
+    for (int i = 0; i < n && i < S::kStages; ++i)
+#pragma unroll
+      for (int a = 0; a < S::kA; ++a) tma_prefetch_3d(&p.w_map, (kb0 + i) * kBlockK, f0, a);
+    for (int s = 0; s < S::kStages; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1);
+    }
+    mbar_init(acc, 1);
+    *failed = 0u;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(slot, S::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *slot_ptr;
+  // only now: a dependent's CTA that started sooner could take the TMEM columns that a CTA
+  // of this launch on the same SM still waits for, and then wait for this launch to end
+  pdl_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      pdl_wait();
+      const uint64_t stream_once = policy_evict_first(), keep = policy_evict_last();
+      int i = 0;
+      for (; i < n; ++i) {
+        const int s = i % S::kStages;
+        if (i >= S::kStages &&
+            !mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty))
+          break;
+        const uint32_t stage = ring + s * S::kStageBytes;
+        mbar_expect_tx(full + 8 * s, S::kStageBytes);
+        const int k = (kb0 + i) * kBlockK;
+#pragma unroll
+        for (int a = 0; a < S::kA; ++a)
+          tma_load_3d(stage + a * kBoxBytes, &p.w_map, k, f0, a, full + 8 * s, gridDim.y > 1 ? keep : stream_once);
+        tma_load_2d(stage + S::kA * kBoxBytes, &p.x_map, k, t0, full + 8 * s, keep);
+      }
+      // leave no copy in flight, whatever ended the loop
+      for (int j = max(0, i - S::kStages); j < i; ++j) mbar_wait_drain(full + 8 * (j % S::kStages), (j / S::kStages) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_i8(kRowsM, BN);
+      for (int i = 0; i < n; ++i) {
+        const int s = i % S::kStages;
+        if (!mbar_wait(full + 8 * s, (i / S::kStages) & 1, &g_int8_error, kErrTimeoutFull)) {
+          *failed = 1u;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t stage = ring + s * S::kStageBytes;
+        const uint64_t b = smem_desc(stage + S::kA * kBoxBytes, 16, 1024, kLayoutSw128);
+#pragma unroll
+        for (int a = 0; a < S::kA; ++a) {
+          const uint64_t w = smem_desc(stage + a * kBoxBytes, 16, 1024, kLayoutSw128);
+#pragma unroll
+          for (int k = 0; k < kBlockK / 32; ++k)  // 32 bytes of depth an instruction
+            tc_mma_i8(tmem + a * BN, w + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
+        }
+        tc_commit(empty + 8 * s);
+      }
+      tc_commit(acc);
+      mbar_wait_drain(acc, 0);
+    }
+    __syncwarp();
+  }
+
+  // Every warp takes part in the reduction; warps 2..5 first bring the sums from TMEM (warp w
+  // reads lanes 32 (w % 4) and on: weight rows) into the ring's place, token-major.
+  pdl_wait();
+  const int live = min(BN, p.tokens - t0);
+  const int width = p.out_type == MM_DTYPE_FP32 ? 16 : 8;
+  const int es = p.out_type == MM_DTYPE_FP32 ? 4 : 2;
+  const bool wide = reinterpret_cast<uintptr_t>(p.out) % width == 0 && p.ld_out * es % width == 0;
+  const int f = f0 + 4 * lane;
+  const int left = p.features - f;
+  float ws[S::kA][4], bias[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int a = 0; a < S::kA; ++a) ws[a][i] = i < left ? p.w_scale[static_cast<int64_t>(a) * p.features + f + i] : 0.0f;
+    bias[i] = p.bias && i < left ? p.bias[f + i] : 0.0f;
+  }
+  bool ok = mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc);
+  tc_fence_after();
+  ok = ok && *failed == 0u;
+  for (int c0 = 0; c0 < live; c0 += S::kChunk) {
+    const int count = min(S::kChunk, live - c0);
+    if (warp >= 2) {
+      const int q = warp & 3;
+#pragma unroll 1
+      for (int j = 0; j < count; j += 16) {
+#pragma unroll
+        for (int a = 0; a < S::kA; ++a) {
+          uint32_t r[16];
+          tc_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + a * BN + c0 + j, r);
+          tc_wait_ld();
+          uint32_t *to = reinterpret_cast<uint32_t *>(ring_ptr) + (j * S::kA + a) * kRowsM + q * 32 + lane;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) to[i * S::kA * kRowsM] = r[i];
+        }
+      }
+    }
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+#pragma unroll 1
+    for (int j = rank * kStreamWarps + warp; j < count; j += split * kStreamWarps) {
+      int4 sum[S::kA];
+#pragma unroll
+      for (int a = 0; a < S::kA; ++a) {
+        const uint32_t at = ring + ((j * S::kA + a) * kRowsM + 4 * lane) * 4;
+        if (split > 1) {
+          sum[a] = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+          for (int r = 0; r < split; ++r) {
+            const int4 v = cluster_load_v4(cluster_map(at, r));
+            sum[a].x += v.x, sum[a].y += v.y, sum[a].z += v.z, sum[a].w += v.w;
+          }
+        } else {
+          sum[a] = *reinterpret_cast<const int4 *>(ring_ptr + (at - ring));
+        }
+      }
+      const int t = t0 + c0 + j;
+      const float xs = p.x_scale[t];
+      float v[4];
+      const int s0[4] = {sum[0].x, sum[0].y, sum[0].z, sum[0].w};
+      if constexpr (GATED) {
+        const int s1[4] = {sum[1].x, sum[1].y, sum[1].z, sum[1].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          v[i] = gate_up(p, __fmul_rn(__fmul_rn(static_cast<float>(s0[i]), xs), ws[0][i]),
+                         __fmul_rn(__fmul_rn(static_cast<float>(s1[i]), xs), ws[1][i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __fmaf_rn(__fmul_rn(static_cast<float>(s0[i]), xs), ws[0][i], bias[i]);
+      }
+      if (ok && left > 0) store4(p, t * p.ld_out + f, left, v, wide);
+    }
+    // the parts are read: the next chunk may take their place, or the CTA may end
+    if (split > 1) cluster_sync();
+    else __syncthreads();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, S::kCols);
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                             const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                             CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+int encoder(EncodeFn *fn) {
+  static EncodeFn cached = nullptr;
+  if (cached == nullptr) {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+    if (e != cudaSuccess || p == nullptr || q != cudaDriverEntryPointSuccess)
+      return set_error(MM_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    cached = reinterpret_cast<EncodeFn>(p);
+  }
+  *fn = cached;
+  return MM_OK;
+}
+
+// 128 bytes wide boxes of `rows` rows, 128-byte swizzle; out-of-range elements read as zero
+// and are not written, so odd depths, tokens and features need no padding.
+int encode(CUtensorMap *map, CUtensorMapDataType type, int es, const void *base, int64_t cols, int64_t rows_total,
+           int64_t planes, int64_t ld, int box_rows) {
+  EncodeFn fn;
+  if (const int rc = encoder(&fn)) return rc;
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows_total), static_cast<cuuint64_t>(planes)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * es), static_cast<cuuint64_t>(ld * es * rows_total)};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(box_rows), 1u};
+  const cuuint32_t step[3] = {1u, 1u, 1u};
+  const CUresult r = fn(map, type, planes ? 3 : 2, const_cast<void *>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(MM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return MM_OK;
+}
+
+template <typename K>
+cudaError_t raise_smem(K kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev >= 0 && dev < 64 && done[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+  return e;
+}
+
+template <typename K>
+cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, int cluster, void *stream, const Int8Args &a) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+template <int BN, bool GATED>
+cudaError_t launch_stream(Int8Args &a, void *stream) {
+  using S = Stream<BN, GATED>;
+  static bool done[64] = {};
+  const cudaError_t e = raise_smem(int8_stream_kernel<BN, GATED>, S::kSmem, done);
+  if (e != cudaSuccess) return e;
+  const int tiles = (a.features + kRowsM - 1) / kRowsM, token_tiles = (a.tokens + BN - 1) / BN;
+  // enough CTAs for two an SM, each with at least two stages of depth
+  int split = 1;
+  while (split < 8 && static_cast<int64_t>(tiles) * token_tiles * split < 148 && 4 * split <= a.blocks_k) split *= 2;
+  a.split = split;
+  return launch_cluster(int8_stream_kernel<BN, GATED>, dim3(tiles * split, token_tiles), kStreamThreads, S::kSmem, split, stream, a);
+}
+
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+struct Product {
+  const int8_t *x;
+  int64_t ld_x;
+  const float *x_scale;
+  const int8_t *w;
+  int64_t ld_w;
+  const float *w_scale, *bias;
+  void *out;
+  int64_t ld_out;
+  int out_type, tokens, features, depth;  // gated: features of h, w holds twice as many rows
+  bool gated;
+  float clamp;
+};
+
+int check(const char *what, const Product &q) {
+  if (q.tokens < 0 || q.features < 1 || q.depth < 1)
+    return set_error(MM_ERR_INVALID, "%s: %d tokens, %d features, depth %d", what, q.tokens, q.features, q.depth);
+  if (q.tokens >= 1 << 23) return set_error(MM_ERR_UNSUPPORTED, "%s: %d tokens: fewer than 2^23 a call", what, q.tokens);
+  if (q.depth >= 1 << 17)
+    return set_error(MM_ERR_UNSUPPORTED, "%s: depth %d: 32-bit sums hold fewer than 131072 products", what, q.depth);
+  if (q.out_type != MM_DTYPE_BF16 && q.out_type != MM_DTYPE_FP16 && q.out_type != MM_DTYPE_FP32)
+    return set_error(MM_ERR_INVALID, "%s: unknown output type %d", what, q.out_type);
+  if (q.tokens == 0) return MM_OK;
+  if (!q.x || !q.x_scale || !q.w || !q.w_scale || !q.out) return set_error(MM_ERR_INVALID, "%s: null pointer", what);
+  if (q.ld_x < q.depth || q.ld_w < q.depth || q.ld_out < q.features)
+    return set_error(MM_ERR_INVALID, "%s: a row stride below the row's length", what);
+  if (!aligned(q.x, 16) || !aligned(q.w, 16) || q.ld_x % 16 || q.ld_w % 16)
+    return set_error(MM_ERR_INVALID, "%s: int8 rows must start on 16-byte boundaries", what);
+  if (!aligned(q.x_scale, 4) || !aligned(q.w_scale, 4) || !aligned(q.bias, 4) || !aligned(q.out, q.out_type == MM_DTYPE_FP32 ? 4 : 2))
+    return set_error(MM_ERR_INVALID, "%s: a misaligned pointer", what);
+  return MM_OK;
+}
+
+int run(const char *what, const Product &q, void *stream) {
+  Int8Args a;
+  a.x_scale = q.x_scale;
+  a.w_scale = q.w_scale;
+  a.bias = q.bias;
+  a.out = q.out;
+  a.ld_out = q.ld_out;
+  a.tokens = q.tokens;
+  a.features = q.features;
+  a.blocks_k = (q.depth + kBlockK - 1) / kBlockK;
+  a.out_type = q.out_type;
+  a.gated = q.gated;
+  a.has_clamp = q.clamp > 0.0f;
+  a.clamp = q.clamp;
+  int rc = encode(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, q.depth, q.features, q.gated ? 2 : 1, q.ld_w, kRowsM);
+  if (rc) return rc;
+  auto x_map = [&](int rows) { return encode(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, q.depth, q.tokens, 0, q.ld_x, rows); };
+  cudaError_t e;
+  const int most = q.gated ? 128 : 256;
+  int bn = 16;
+  while (bn < q.tokens && bn < most) bn *= 2;
+  if ((rc = x_map(bn))) return rc;
+  switch (q.gated ? -bn : bn) {
+    case 16: e = launch_stream<16, false>(a, stream); break;
+    case 32: e = launch_stream<32, false>(a, stream); break;
+    case 64: e = launch_stream<64, false>(a, stream); break;
+    case 128: e = launch_stream<128, false>(a, stream); break;
+    case 256: e = launch_stream<256, false>(a, stream); break;
+    case -16: e = launch_stream<16, true>(a, stream); break;
+    case -32: e = launch_stream<32, true>(a, stream); break;
+    case -64: e = launch_stream<64, true>(a, stream); break;
+    default: e = launch_stream<128, true>(a, stream); break;
+  }
+  if (e != cudaSuccess) return set_error(MM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+  return MM_OK;
+}
+
+int64_t up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+}  // namespace
+}  // namespace mm
+
+using namespace mm;
+
+extern "C" {
+
+int mm_int8_linear(const int8_t *x, int64_t ld_x, const float *x_scale, const int8_t *w, int64_t ld_w,
+                   const float *w_scale, const float *bias, void *out, int64_t ld_out, int32_t out_dtype,
+                   int32_t tokens, int32_t features, int32_t depth, void *stream) {
+  const Product q = {x, ld_x, x_scale, w, ld_w, w_scale, bias, out, ld_out, out_dtype, tokens, features, depth, false, 0.0f};
+  const int rc = check("mm_int8_linear", q);
+  if (rc || tokens == 0) return rc;
+  return run("mm_int8_linear", q, stream);
+}
+
+int64_t mm_int8_ffn_workspace(int32_t tokens, int32_t inter) {
+  if (tokens < 1 || inter < 1) return 0;
+  return up(static_cast<int64_t>(tokens) * inter * 4, 256) + up(tokens * up(inter, 16), 256) + static_cast<int64_t>(tokens) * 4;
+}
+
+int mm_int8_ffn(const mm_int8_ffn_args *f, void *stream) {
+  if (!f) return set_error(MM_ERR_INVALID, "mm_int8_ffn: null pointer");
+  if (f->clamp < 0.0f || !(f->clamp < INFINITY)) return set_error(MM_ERR_INVALID, "mm_int8_ffn: clamp %g", f->clamp);
+  if (f->tokens < 0 || f->inter < 1 || f->inter >= 1 << 30)
+    return set_error(MM_ERR_INVALID, "mm_int8_ffn: %d tokens, inter %d", f->tokens, f->inter);
+  uint8_t *ws = static_cast<uint8_t *>(f->workspace);
+  if (f->tokens > 0 && (!ws || !aligned(ws, 256) || f->workspace_bytes < mm_int8_ffn_workspace(f->tokens, f->inter)))
+    return set_error(MM_ERR_INVALID, "mm_int8_ffn: the workspace needs %lld bytes on a 256-byte boundary",
+                     static_cast<long long>(mm_int8_ffn_workspace(f->tokens, f->inter)));
+  // h in fp32 (its rounding to int8 is the only one), then its codes and scales
+  const int64_t ld_q = up(f->inter, 16);
+  float *h = reinterpret_cast<float *>(ws);
+  int8_t *hq = ws ? reinterpret_cast<int8_t *>(ws + up(static_cast<int64_t>(f->tokens) * f->inter * 4, 256)) : nullptr;
+  float *hs = ws ? reinterpret_cast<float *>(hq + up(f->tokens * ld_q, 256)) : nullptr;
+  const Product up_q = {f->x, f->ld_x, f->x_scale, f->w13, f->ld_w13, f->w13_scale, nullptr, h, f->inter, MM_DTYPE_FP32,
+                        f->tokens, f->inter, f->hidden, true, f->clamp};
+  const Product down_q = {hq, ld_q, hs, f->w2, f->ld_w2, f->w2_scale, nullptr, f->out, f->ld_out, f->out_dtype,
+                          f->tokens, f->hidden, f->inter, false, 0.0f};
+  int rc = check("mm_int8_ffn", up_q);
+  if (!rc) rc = check("mm_int8_ffn", down_q);
+  if (rc || f->tokens == 0) return rc;
+  if ((rc = run("mm_int8_ffn", up_q, stream))) return rc;
+  if ((rc = quantize_rows("mm_int8_ffn", h, f->inter, MM_DTYPE_FP32, hq, ld_q, hs, f->tokens, f->inter, stream))) return rc;
+  return run("mm_int8_ffn", down_q, stream);
+}
+
+int mm_int8_check(void) {
+  cudaError_t e = cudaDeviceSynchronize();
+  uint32_t word = 0;
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&word, g_int8_error, sizeof(word));
+  if (e == cudaSuccess && word) {
+    const uint32_t zero = 0;
+    e = cudaMemcpyToSymbol(g_int8_error, &zero, sizeof(zero));
+  }
+  if (e != cudaSuccess) return set_error(MM_ERR_CUDA, "mm_int8_check: %s", cudaGetErrorString(e));
+  if (word) return set_error(MM_ERR_DEVICE_TIMEOUT, "device wait timed out (error word 0x%x)", word);
+  return MM_OK;
+}
+
+}  // extern "C"

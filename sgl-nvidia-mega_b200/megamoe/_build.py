@@ -17,8 +17,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
 REPO = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
-SOURCES = ["mm_api.cu", "mm_route.cu", "mm_gate_dsv41.cu", "mm_experts.cu", "mm_finalize.cu", "mm_comm.cu"]
-HEADERS = ["mm_gate.cuh", "mm_kernels.cuh", "mm_layout.cuh", "mm_numerics.cuh", "mm_ptx.cuh"]
+SOURCES = ["mm_api.cu", "mm_route.cu", "mm_gate_dsv41.cu", "mm_experts.cu", "mm_finalize.cu", "mm_comm.cu", "mm_norm.cu",
+           "mm_int8.cu"]
+HEADERS = ["mm_dense.cuh", "mm_gate.cuh", "mm_kernels.cuh", "mm_layout.cuh", "mm_numerics.cuh", "mm_ptx.cuh"]
 OUTPUT = os.path.join(HERE, "libmegamoe.so")
 OBJDIR = os.path.join(HERE, "_build")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")

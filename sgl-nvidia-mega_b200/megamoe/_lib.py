@@ -38,6 +38,14 @@ RENORMS = {"none": MM_RENORM_NONE, "sum": MM_RENORM_SUM, "scaled_bf16": MM_RENOR
 MM_WEIGHT_MXFP4 = 0
 MM_WEIGHT_NVFP4 = 1
 
+MM_DTYPE_BF16 = 0
+MM_DTYPE_FP16 = 1
+MM_DTYPE_FP32 = 2
+
+MM_QUANT_NONE = 0
+MM_QUANT_MXFP8 = 1
+MM_QUANT_INT8 = 2
+
 MM_SCRATCH_X_CODES = 0
 MM_SCRATCH_X_SCALES = 1
 MM_SCRATCH_H_CODES = 2
@@ -152,6 +160,52 @@ class MMStackLayer(ctypes.Structure):
     _fields_ = [("layer", c_void_p), ("args", MMForwardArgs)]
 
 
+class MMNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("residual", c_void_p),
+        ("gamma", c_void_p),
+        ("residual_out", c_void_p),
+        ("norm_out", c_void_p),
+        ("codes", c_void_p),
+        ("scales", c_void_p),
+        ("ld_x", c_int64),
+        ("ld_residual", c_int64),
+        ("ld_residual_out", c_int64),
+        ("ld_norm", c_int64),
+        ("ld_codes", c_int64),
+        ("tokens", c_int32),
+        ("hidden", c_int32),
+        ("dtype", c_int32),
+        ("gamma_dtype", c_int32),
+        ("quant", c_int32),
+        ("eps", c_float),
+    ]
+
+
+class MMInt8FFNArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", c_void_p),
+        ("x_scale", c_void_p),
+        ("w13", c_void_p),
+        ("w13_scale", c_void_p),
+        ("w2", c_void_p),
+        ("w2_scale", c_void_p),
+        ("out", c_void_p),
+        ("workspace", c_void_p),
+        ("workspace_bytes", c_int64),
+        ("ld_x", c_int64),
+        ("ld_w13", c_int64),
+        ("ld_w2", c_int64),
+        ("ld_out", c_int64),
+        ("tokens", c_int32),
+        ("hidden", c_int32),
+        ("inter", c_int32),
+        ("out_dtype", c_int32),
+        ("clamp", c_float),
+    ]
+
+
 # name -> (restype, argtypes); every extern "C" symbol of include/megamoe.h
 SIGNATURES = {
     "mm_last_error": (ctypes.c_char_p, []),
@@ -164,6 +218,19 @@ SIGNATURES = {
         c_int32,
         [POINTER(MMGateArgs), c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p],
     ),
+    "mm_rms_norm": (c_int32, [POINTER(MMNormArgs), c_void_p]),
+    "mm_quantize_int8": (
+        c_int32,
+        [c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p, c_int32, c_int32, c_void_p],
+    ),
+    "mm_int8_linear": (
+        c_int32,
+        [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_int32,
+         c_int32, c_int32, c_void_p],
+    ),
+    "mm_int8_ffn_workspace": (c_int64, [c_int32, c_int32]),
+    "mm_int8_ffn": (c_int32, [POINTER(MMInt8FFNArgs), c_void_p]),
+    "mm_int8_check": (c_int32, []),
     "mm_finalize": (
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p],
