@@ -38,6 +38,9 @@ constexpr int kBlockK = 128;          // depth of a stage, bytes
 constexpr int kRowsM = 128;           // weight rows of a box, token rows of a pair's half
 constexpr int kBoxBytes = kRowsM * kBlockK;
 
+// Above this many tokens the tile form takes over.
+constexpr int kTileTokens = 256;
+
 // Error word of this file's launches: bounded waits that ran out (mm_int8_check).
 __device__ uint32_t g_int8_error;
 
@@ -50,11 +53,12 @@ struct alignas(64) Int8Args {
   int64_t ld_out;
   int tokens, features, blocks_k;
   int out_type;
-  int stage_out;        // output rows start on 16-byte boundaries: TMA stores
+  int stage_out;        // output rows start and end on 16-byte boundaries: TMA stores (a store
+                        // that ends inside a 16-byte unit also writes the rest of the unit)
   int gated;
   int has_clamp;
   float clamp;
-  int token_tiles, feature_tiles;  // of the tile form
+  int token_tiles, feature_tiles, tile_n;  // of the tile form
   int split;            // CTAs of a cluster that share a tile's depth (stream form)
 };
 
@@ -294,6 +298,234 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
 }
 
 // ---------------------------------------------------------------------------------------
+// The tile form. Per CTA: warp 0 loads, warp 1 (of the pair's leader) issues the products,
+// warps 2..5 are the epilogue; every warp of both CTAs walks the same tiles.
+constexpr int kTileM = 256;                        // tokens of a pair
+constexpr int kTileN = 256;                        // weight rows of a pair at most
+constexpr int kTileStages = 6;
+constexpr int kTileStageBytes = 2 * kBoxBytes;     // this CTA's halves of both operands
+constexpr int kTileThreads = 192;
+constexpr int kOutChunk = 32;                      // columns of one TMEM read and one store
+constexpr int kOutBytes = 32 * kOutChunk * 4;      // a warp's staged chunk (32 rows), fp32
+constexpr int kTileSmem = 1024 + kTileStages * kTileStageBytes + 4 * kOutBytes + 4 * 2 * kTileN * 4 + 256;
+
+// The tile of a step: token tiles in groups of 16 (their codes stay in L2 while the weights
+// pass by once a group), fastest inside a group.
+__device__ __forceinline__ void tile_at(const Int8Args &p, int i, int &tt, int &ft) {
+  const int per = 16 * p.feature_tiles;
+  const int g = i / per, r = i - g * per;
+  const int rows = min(16, p.token_tiles - 16 * g);
+  ft = r / rows;
+  tt = 16 * g + r - ft * rows;
+}
+
+template <typename Out, bool GATED>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int8_tile_kernel(const __grid_constant__ Int8Args p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t ring = (raw + 1023u) & ~1023u;
+  uint8_t *base = smem_raw + (ring - raw);
+  const uint32_t out_stage = ring + kTileStages * kTileStageBytes;
+  float *scales = reinterpret_cast<float *>(base + kTileStages * kTileStageBytes + 4 * kOutBytes);
+  const uint32_t bars = out_stage + 4 * kOutBytes + 4 * 2 * kTileN * 4;
+  const uint32_t full = bars, empty = full + 8 * kTileStages, acc_full = empty + 8 * kTileStages,
+                 acc_empty = acc_full + 16, drained = acc_empty + 16, slot = drained + 8;
+  uint32_t *slot_ptr = reinterpret_cast<uint32_t *>(base + (slot - ring));
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_rank());
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int tiles = p.token_tiles * p.feature_tiles;
+  const int half_n = p.tile_n / 2;                 // weight rows that this CTA stages
+  const int tile_f = GATED ? half_n : p.tile_n;    // features of a tile
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&p.w_map);
+    tma_prefetch_desc(&p.x_map);
+    if (p.stage_out) tma_prefetch_desc(&p.out_map);
+    for (int s = 0; s < kTileStages; ++s) {
+      mbar_init(full + 8 * s, 1);
+      mbar_init(empty + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full + 8 * b, 1);
+      mbar_init(acc_empty + 8 * b, 8);  // four epilogue warps of either CTA
+    }
+    mbar_init(drained, 1);
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_pair_alloc(slot, 512);
+    tmem_pair_relinquish();
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *slot_ptr;
+  pdl_launch_dependents();  // after the allocation, as in the stream form
+
+  if (warp == 0) {
+    if (lane == 0) {
+      pdl_wait();
+      const uint32_t stage_tx = 2 * (kBoxBytes + half_n * kBlockK);  // both CTAs' bytes
+      int it = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        int tt, ft;
+        tile_at(p, tile, tt, ft);
+        const int t0 = tt * kTileM + rank * kRowsM;
+        const int row = GATED ? ft * tile_f : ft * tile_f + rank * half_n, plane = GATED ? rank : 0;
+        for (int kb = 0; kb < p.blocks_k; ++kb, ++it) {
+          const int s = it % kTileStages;
+          if (it >= kTileStages &&
+              !mbar_wait_cluster(empty + 8 * s, ((it / kTileStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          const uint32_t stage = ring + s * kTileStageBytes;
+          // the leader's barrier counts the bytes of both CTAs: this CTA's copies may land
+          // there before the leader expects them, the phase still ends with its arrival
+          const uint32_t bar = cluster_map(full + 8 * s, 0);
+          if (rank == 0) mbar_expect_tx(full + 8 * s, stage_tx);
+          tma_pair_load_2d(stage, &p.x_map, kb * kBlockK, t0, bar);
+          tma_pair_load_3d(stage + kBoxBytes, &p.w_map, kb * kBlockK, row, plane, bar);
+        }
+      }
+      // leave no copy in flight: the last stages' barriers complete with both CTAs' copies
+      if (rank == 0)
+        for (int j = max(0, it - kTileStages); j < it; ++j)
+          mbar_wait_drain(full + 8 * (j % kTileStages), (j / kTileStages) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = idesc_i8(kTileM, p.tile_n);
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int tile = pair; tile < tiles && ok; tile += pairs, ++n) {
+        const int b = n & 1;
+        if (n >= 2 && !mbar_wait_cluster(acc_empty + 8 * b, ((n >> 1) - 1) & 1, &g_int8_error, kErrTimeoutAcc)) break;
+        tc_fence_after();
+        for (int kb = 0; kb < p.blocks_k; ++kb, ++it) {
+          const int s = it % kTileStages;
+          if (!mbar_wait_cluster(full + 8 * s, (it / kTileStages) & 1, &g_int8_error, kErrTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t stage = ring + s * kTileStageBytes;
+          const uint64_t x = smem_desc(stage, 16, 1024, kLayoutSw128);
+          const uint64_t w = smem_desc(stage + kBoxBytes, 16, 1024, kLayoutSw128);
+#pragma unroll
+          for (int k = 0; k < kBlockK / 32; ++k) tc_pair_mma_i8(tmem + b * kTileN, x + 2 * k, w + 2 * k, idesc, kb > 0 || k > 0);
+          tc_pair_commit(empty + 8 * s);
+        }
+        if (ok) tc_pair_commit(acc_full + 8 * b);
+      }
+      tc_pair_commit(drained);
+      mbar_wait_drain(drained, 0);
+    }
+    __syncwarp();
+  } else {
+    pdl_wait();
+    const int q = warp & 3;  // TMEM lanes 32 q and on: token rows
+    float *ws = scales + q * 2 * kTileN, *second = ws + kTileN;  // second: the bias, or the up rows' scales
+    const uint32_t mine = out_stage + q * kOutBytes;
+    int n = 0;
+    for (int tile = pair; tile < tiles; tile += pairs, ++n) {
+      const int b = n & 1;
+      int tt, ft;
+      tile_at(p, tile, tt, ft);
+      const int t0 = tt * kTileM + rank * kRowsM + q * 32, t = t0 + lane;
+      const int f0 = ft * tile_f;
+      const float xs = t < p.tokens ? p.x_scale[t] : 0.0f;
+      __syncwarp();
+      for (int i = lane; i < tile_f; i += 32) {
+        const bool in = f0 + i < p.features;
+        ws[i] = in ? p.w_scale[f0 + i] : 0.0f;
+        second[i] = !in ? 0.0f : GATED ? p.w_scale[p.features + f0 + i] : p.bias ? p.bias[f0 + i] : 0.0f;
+      }
+      __syncwarp();
+      if (!mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc)) break;
+      tc_fence_after();
+      const uint32_t from = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kTileN;
+      for (int c = 0; c < tile_f; c += kOutChunk) {
+        uint32_t r[kOutChunk], u[GATED ? kOutChunk : 1];
+        tc_ld_32x32b_x32(from + c, r);
+        if constexpr (GATED) tc_ld_32x32b_x32(from + half_n + c, u);
+        tc_wait_ld();
+        if (c + kOutChunk == tile_f) {
+          // the accumulator is in registers: the pair's next but one tile may overwrite it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(cluster_map(acc_empty + 8 * b, 0));
+        }
+        float v[kOutChunk];
+#pragma unroll
+        for (int j = 0; j < kOutChunk; j += 4) {
+          const float4 w4 = *reinterpret_cast<const float4 *>(ws + c + j), s4 = *reinterpret_cast<const float4 *>(second + c + j);
+          const float w[4] = {w4.x, w4.y, w4.z, w4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float a = __fmul_rn(static_cast<float>(static_cast<int>(r[j + i])), xs);
+            if constexpr (GATED)
+              v[j + i] = gate_up(p, __fmul_rn(a, w[i]), __fmul_rn(__fmul_rn(static_cast<float>(static_cast<int>(u[j + i])), xs), s[i]));
+            else
+              v[j + i] = __fmaf_rn(a, w[i], s[i]);
+          }
+        }
+        if (p.stage_out) {
+          // this warp's [32 rows][32 columns], swizzled as the map says (16-byte units XORed
+          // with the row so that eight lanes' stores touch eight banks' units), then one store
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+          uint8_t *row = base + (mine - ring);
+          if constexpr (sizeof(Out) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<float4 *>(row + lane * 128 + ((i ^ (lane & 7)) * 16)) =
+                  make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              union { uint4 w; Out h[8]; } pk;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) pk.h[j] = Out(v[8 * i + j]);
+              *reinterpret_cast<uint4 *>(row + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)) = pk.w;
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && t0 < p.tokens && f0 + c < p.features) {
+            tma_store_2d(&p.out_map, mine, f0 + c, t0);
+            bulk_commit_group();
+          }
+        } else {
+          // rows that TMA cannot store: turned in shared memory (columns XORed with the row: no
+          // bank meets twice), then a row of 32 columns an instruction
+          float *turn = reinterpret_cast<float *>(base + (mine - ring));
+#pragma unroll
+          for (int i = 0; i < kOutChunk; ++i) turn[lane * 32 + (i ^ lane)] = v[i];
+          __syncwarp();
+          const int rows = min(32, p.tokens - t0);
+          if (f0 + c + lane < p.features) {
+            Out *o = static_cast<Out *>(p.out) + t0 * p.ld_out + f0 + c + lane;
+#pragma unroll 8
+            for (int j = 0; j < rows; ++j, o += p.ld_out) *o = Out(turn[j * 32 + (lane ^ j)]);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) tmem_pair_dealloc(tmem, 512);
+}
+
+// ---------------------------------------------------------------------------------------
 // Host side
 typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                              const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
@@ -313,19 +545,20 @@ int encoder(EncodeFn *fn) {
   return MM_OK;
 }
 
-// 128 bytes wide boxes of `rows` rows, 128-byte swizzle; out-of-range elements read as zero
+// Boxes of 128 (or 64) bytes by `box_rows` rows with the swizzle of that width; out-of-range elements read as zero
 // and are not written, so odd depths, tokens and features need no padding.
 int encode(CUtensorMap *map, CUtensorMapDataType type, int es, const void *base, int64_t cols, int64_t rows_total,
-           int64_t planes, int64_t ld, int box_rows) {
+           int64_t planes, int64_t ld, int box_rows, int box_bytes = 128) {
   EncodeFn fn;
   if (const int rc = encoder(&fn)) return rc;
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows_total), static_cast<cuuint64_t>(planes)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld * es), static_cast<cuuint64_t>(ld * es * rows_total)};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(128 / es), static_cast<cuuint32_t>(box_rows), 1u};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(box_bytes / es), static_cast<cuuint32_t>(box_rows), 1u};
   const cuuint32_t step[3] = {1u, 1u, 1u};
   const CUresult r = fn(map, type, planes ? 3 : 2, const_cast<void *>(base), dims, strides, box, step,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(MM_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
   return MM_OK;
 }
@@ -371,6 +604,45 @@ cudaError_t launch_stream(Int8Args &a, void *stream) {
   while (split < 8 && static_cast<int64_t>(tiles) * token_tiles * split < 148 && 4 * split <= a.blocks_k) split *= 2;
   a.split = split;
   return launch_cluster(int8_stream_kernel<BN, GATED>, dim3(tiles * split, token_tiles), kStreamThreads, S::kSmem, split, stream, a);
+}
+
+// CTA pairs that the current device runs at once (of the tile form: one CTA an SM, all its
+// forms alike), the persistent grid's size. 0: not known.
+int sm_pairs() {
+  static int cached[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (!cached[dev]) {
+    static bool done[64] = {};
+    if (raise_smem(int8_tile_kernel<float, true>, kTileSmem, done) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(256);
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = kTileSmem;
+    int clusters = 0;
+    if (cudaOccupancyMaxActiveClusters(&clusters, int8_tile_kernel<float, true>, &cfg) != cudaSuccess) return 0;
+    cached[dev] = clusters;
+  }
+  return cached[dev];
+}
+
+template <typename Out, bool GATED>
+cudaError_t launch_tile(Int8Args &a, int pairs, void *stream) {
+  static bool done[64] = {};
+  const cudaError_t e = raise_smem(int8_tile_kernel<Out, GATED>, kTileSmem, done);
+  if (e != cudaSuccess) return e;
+  const int tiles = a.token_tiles * a.feature_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * std::min(tiles, pairs));
+  cfg.blockDim = dim3(kTileThreads);
+  cfg.dynamicSmemBytes = kTileSmem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, int8_tile_kernel<Out, GATED>, a);
 }
 
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -422,10 +694,38 @@ int run(const char *what, const Product &q, void *stream) {
   a.gated = q.gated;
   a.has_clamp = q.clamp > 0.0f;
   a.clamp = q.clamp;
-  int rc = encode(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, q.depth, q.features, q.gated ? 2 : 1, q.ld_w, kRowsM);
-  if (rc) return rc;
+  auto w_map = [&](int rows) { return encode(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, q.depth, q.features, q.gated ? 2 : 1, q.ld_w, rows); };
+  int rc;
   auto x_map = [&](int rows) { return encode(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, q.depth, q.tokens, 0, q.ld_x, rows); };
   cudaError_t e;
+  const int pairs = q.tokens > kTileTokens ? sm_pairs() : 0;
+  if (pairs > 0) {
+    // the width that leaves the pairs the least to do, an epilogue counted as 32 columns
+    int64_t best = INT64_MAX;
+    a.token_tiles = (q.tokens + kTileM - 1) / kTileM;
+    for (int n = kTileN; n >= 64; n -= q.gated ? 64 : 32) {
+      const int f = q.gated ? n / 2 : n;
+      const int64_t tiles = static_cast<int64_t>(a.token_tiles) * ((q.features + f - 1) / f);
+      const int64_t cost = (tiles + pairs - 1) / pairs * (n + 32);
+      if (cost < best) best = cost, a.tile_n = n, a.feature_tiles = (q.features + f - 1) / f;
+    }
+    const int es = q.out_type == MM_DTYPE_FP32 ? 4 : 2;
+    a.stage_out = aligned(q.out, 16) && q.ld_out * es % 16 == 0 && static_cast<int64_t>(q.features) * es % 16 == 0;
+    if ((rc = x_map(kRowsM)) || (rc = w_map(a.tile_n / 2))) return rc;
+    if (a.stage_out &&
+        (rc = encode(&a.out_map, q.out_type == MM_DTYPE_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                 : q.out_type == MM_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                     es, q.out, q.features, q.tokens, 0, q.ld_out, 32, kOutChunk * es)))
+      return rc;
+    if (q.gated) e = launch_tile<float, true>(a, pairs, stream);
+    else if (q.out_type == MM_DTYPE_FP32) e = launch_tile<float, false>(a, pairs, stream);
+    else if (q.out_type == MM_DTYPE_BF16) e = launch_tile<__nv_bfloat16, false>(a, pairs, stream);
+    else e = launch_tile<__half, false>(a, pairs, stream);
+    if (e != cudaSuccess) return set_error(MM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    return MM_OK;
+  }
+  if ((rc = w_map(kRowsM))) return rc;
   const int most = q.gated ? 128 : 256;
   int bn = 16;
   while (bn < q.tokens && bn < most) bn *= 2;

@@ -281,8 +281,8 @@ __device__ __forceinline__ uint32_t cluster_size() {
 }
 // Every thread of every CTA of the cluster; orders shared-memory accesses across it.
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
 // The address of this CTA's shared-memory location `addr` in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t cluster_map(uint32_t addr, uint32_t rank) {
@@ -369,6 +369,35 @@ __device__ __forceinline__ void tc_pair_mma_i8(uint32_t d_tmem, uint64_t adesc, 
       "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+// mbar_wait on a barrier that the other CTA of the pair arrives on too.
+__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0u;
+}
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint32_t *err, uint32_t code) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+  const uint64_t t0 = globaltimer();
+#pragma unroll 1
+  for (uint32_t i = 0;; ++i) {
+    if (mbar_try_wait_cluster(bar, parity)) return true;
+    if ((i & 63u) == 0u) {
+      if (error_set(err)) return false;
+      if (globaltimer() - t0 > kWaitBudgetNs) {
+        error_raise(err, code);
+        return false;
+      }
+    }
+  }
 }
 // Arrive on `bar` of both CTAs of the pair once every MMA this thread issued has completed.
 __device__ __forceinline__ void tc_pair_commit(uint32_t bar) {
