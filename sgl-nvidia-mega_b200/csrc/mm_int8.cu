@@ -62,6 +62,9 @@ struct alignas(64) Int8Args {
   int split;            // CTAs of a cluster that share a tile's depth (stream form)
 };
 
+// A whole warp waits, one elected lane issues: the lanes go on together, or give up together.
+__device__ __forceinline__ bool warp_agrees(bool ok) { return __all_sync(0xffffffffu, ok); }
+
 __device__ __forceinline__ float gate_up(const Int8Args &p, float g, float u) {
   if (p.has_clamp) {
     // NaN stays NaN: comparisons instead of fminf / fmaxf
@@ -169,49 +172,56 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   pdl_launch_dependents();
 
   if (warp == 0) {
-    if (lane == 0) {
+    {
       pdl_wait();
       const uint64_t stream_once = policy_evict_first(), keep = policy_evict_last();
       int i = 0;
       for (; i < n; ++i) {
         const int s = i % S::kStages;
         if (i >= S::kStages &&
-            !mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty))
+            !warp_agrees(mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty)))
           break;
         const uint32_t stage = ring + s * S::kStageBytes;
-        mbar_expect_tx(full + 8 * s, S::kStageBytes);
         const int k = (kb0 + i) * kBlockK;
+        if (elect_one()) {
+          mbar_expect_tx(full + 8 * s, S::kStageBytes);
 #pragma unroll
-        for (int a = 0; a < S::kA; ++a)
-          tma_load_3d(stage + a * kBoxBytes, &p.w_map, k, f0, a, full + 8 * s, gridDim.y > 1 ? keep : stream_once);
-        tma_load_2d(stage + S::kA * kBoxBytes, &p.x_map, k, t0, full + 8 * s, keep);
+          for (int a = 0; a < S::kA; ++a)
+            tma_load_3d(stage + a * kBoxBytes, &p.w_map, k, f0, a, full + 8 * s, gridDim.y > 1 ? keep : stream_once);
+          tma_load_2d(stage + S::kA * kBoxBytes, &p.x_map, k, t0, full + 8 * s, keep);
+        }
+        __syncwarp();
       }
       // leave no copy in flight, whatever ended the loop
       for (int j = max(0, i - S::kStages); j < i; ++j) mbar_wait_drain(full + 8 * (j % S::kStages), (j / S::kStages) & 1);
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    {
       constexpr uint32_t idesc = idesc_i8(kRowsM, BN);
       for (int i = 0; i < n; ++i) {
         const int s = i % S::kStages;
-        if (!mbar_wait(full + 8 * s, (i / S::kStages) & 1, &g_int8_error, kErrTimeoutFull)) {
+        if (!warp_agrees(mbar_wait(full + 8 * s, (i / S::kStages) & 1, &g_int8_error, kErrTimeoutFull))) {
           *failed = 1u;
           break;
         }
         tc_fence_after();
         const uint32_t stage = ring + s * S::kStageBytes;
         const uint64_t b = smem_desc(stage + S::kA * kBoxBytes, 16, 1024, kLayoutSw128);
+        if (elect_one()) {
 #pragma unroll
-        for (int a = 0; a < S::kA; ++a) {
-          const uint64_t w = smem_desc(stage + a * kBoxBytes, 16, 1024, kLayoutSw128);
+          for (int a = 0; a < S::kA; ++a) {
+            const uint64_t w = smem_desc(stage + a * kBoxBytes, 16, 1024, kLayoutSw128);
 #pragma unroll
-          for (int k = 0; k < kBlockK / 32; ++k)  // 32 bytes of depth an instruction
-            tc_mma_i8(tmem + a * BN, w + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
+            for (int k = 0; k < kBlockK / 32; ++k)  // 32 bytes of depth an instruction
+              tc_mma_i8(tmem + a * BN, w + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
+          }
+          tc_commit(empty + 8 * s);
         }
-        tc_commit(empty + 8 * s);
+        __syncwarp();
       }
-      tc_commit(acc);
+      if (elect_one()) tc_commit(acc);
+      __syncwarp();
       mbar_wait_drain(acc, 0);
     }
     __syncwarp();
@@ -365,7 +375,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
   pdl_launch_dependents();  // after the allocation, as in the stream form
 
   if (warp == 0) {
-    if (lane == 0) {
+    {
       pdl_wait();
       const uint32_t stage_tx = 2 * (kBoxBytes + half_n * kBlockK);  // both CTAs' bytes
       int it = 0;
@@ -378,7 +388,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
         for (int kb = 0; kb < p.blocks_k; ++kb, ++it) {
           const int s = it % kTileStages;
           if (it >= kTileStages &&
-              !mbar_wait_cluster(empty + 8 * s, ((it / kTileStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty)) {
+              !warp_agrees(mbar_wait_cluster(empty + 8 * s, ((it / kTileStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty))) {
             ok = false;
             break;
           }
@@ -386,9 +396,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
           // the leader's barrier counts the bytes of both CTAs: this CTA's copies may land
           // there before the leader expects them, the phase still ends with its arrival
           const uint32_t bar = cluster_map(full + 8 * s, 0);
-          if (rank == 0) mbar_expect_tx(full + 8 * s, stage_tx);
-          tma_pair_load_2d(stage, &p.x_map, kb * kBlockK, t0, bar);
-          tma_pair_load_3d(stage + kBoxBytes, &p.w_map, kb * kBlockK, row, plane, bar);
+          if (elect_one()) {
+            if (rank == 0) mbar_expect_tx(full + 8 * s, stage_tx);
+            tma_pair_load_2d(stage, &p.x_map, kb * kBlockK, t0, bar);
+            tma_pair_load_3d(stage + kBoxBytes, &p.w_map, kb * kBlockK, row, plane, bar);
+          }
+          __syncwarp();
         }
       }
       // leave no copy in flight: the last stages' barriers complete with both CTAs' copies
@@ -398,17 +411,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       const uint32_t idesc = idesc_i8(kTileM, p.tile_n);
       int it = 0, n = 0;
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += pairs, ++n) {
         const int b = n & 1;
-        if (n >= 2 && !mbar_wait_cluster(acc_empty + 8 * b, ((n >> 1) - 1) & 1, &g_int8_error, kErrTimeoutAcc)) break;
+        if (n >= 2 && !warp_agrees(mbar_wait_cluster(acc_empty + 8 * b, ((n >> 1) - 1) & 1, &g_int8_error, kErrTimeoutAcc))) break;
         tc_fence_after();
         for (int kb = 0; kb < p.blocks_k; ++kb, ++it) {
           const int s = it % kTileStages;
-          if (!mbar_wait_cluster(full + 8 * s, (it / kTileStages) & 1, &g_int8_error, kErrTimeoutFull)) {
+          if (!warp_agrees(mbar_wait_cluster(full + 8 * s, (it / kTileStages) & 1, &g_int8_error, kErrTimeoutFull))) {
             ok = false;
             break;
           }
@@ -416,13 +429,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
           const uint32_t stage = ring + s * kTileStageBytes;
           const uint64_t x = smem_desc(stage, 16, 1024, kLayoutSw128);
           const uint64_t w = smem_desc(stage + kBoxBytes, 16, 1024, kLayoutSw128);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kBlockK / 32; ++k) tc_pair_mma_i8(tmem + b * kTileN, x + 2 * k, w + 2 * k, idesc, kb > 0 || k > 0);
-          tc_pair_commit(empty + 8 * s);
+            for (int k = 0; k < kBlockK / 32; ++k) tc_pair_mma_i8(tmem + b * kTileN, x + 2 * k, w + 2 * k, idesc, kb > 0 || k > 0);
+            tc_pair_commit(empty + 8 * s);
+          }
+          __syncwarp();
         }
-        if (ok) tc_pair_commit(acc_full + 8 * b);
+        if (ok && elect_one()) tc_pair_commit(acc_full + 8 * b);
+        __syncwarp();
       }
-      tc_pair_commit(drained);
+      if (elect_one()) tc_pair_commit(drained);
+      __syncwarp();
       mbar_wait_drain(drained, 0);
     }
     __syncwarp();
@@ -446,7 +464,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
         second[i] = !in ? 0.0f : GATED ? p.w_scale[p.features + f0 + i] : p.bias ? p.bias[f0 + i] : 0.0f;
       }
       __syncwarp();
-      if (!mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc)) break;
+      if (!warp_agrees(mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc))) break;
       tc_fence_after();
       const uint32_t from = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kTileN;
       for (int c = 0; c < tile_f; c += kOutChunk) {

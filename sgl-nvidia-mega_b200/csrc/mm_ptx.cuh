@@ -268,6 +268,19 @@ __device__ __forceinline__ uint32_t idesc_mxf4_e4m3(uint32_t n, uint32_t a_sf_id
   return d;
 }
 
+// One lane of a converged warp (true for it alone). The compiler knows that a branch on it has
+// one thread, and issues the tcgen05 and TMA instructions inside without the loop over
+// lanes that a branch on the lane number costs them.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(p));
+  return p != 0u;
+}
+
 // ---- thread-block clusters ------------------------------------------------------
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
