@@ -312,8 +312,13 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
 // warps 2..5 are the epilogue; every warp of both CTAs walks the same tiles.
 constexpr int kTileM = 256;                        // tokens of a pair
 constexpr int kTileN = 256;                        // weight rows of a pair at most
-constexpr int kTileStages = 6;
-constexpr int kTileStageBytes = 2 * kBoxBytes;     // this CTA's halves of both operands
+// A stage is two blocks of depth, 64 KB of this CTA's halves of both operands: a hand-over
+// (full barrier, commit, empty barrier) costs about 225 ns whatever it hands over, a block's
+// products 266 ns at 256 columns and 66 at 64. One block a stage: 128 columns 439 us against
+// 324 at 8192 x 7168 x 7168, 256 columns the same.
+constexpr int kTileBlocks = 2;
+constexpr int kTileStages = 3;
+constexpr int kTileStageBytes = kTileBlocks * 2 * kBoxBytes;
 constexpr int kTileThreads = 192;
 constexpr int kOutChunk = 32;                      // columns of one TMEM read and one store
 constexpr int kOutBytes = 32 * kOutChunk * 4;      // a warp's staged chunk (32 rows), fp32
@@ -377,7 +382,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
   if (warp == 0) {
     {
       pdl_wait();
-      const uint32_t stage_tx = 2 * (kBoxBytes + half_n * kBlockK);  // both CTAs' bytes
+      const uint32_t block_tx = 2 * (kBoxBytes + half_n * kBlockK);  // both CTAs' bytes
       int it = 0;
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += pairs) {
@@ -385,7 +390,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
         tile_at(p, tile, tt, ft);
         const int t0 = tt * kTileM + rank * kRowsM;
         const int row = GATED ? ft * tile_f : ft * tile_f + rank * half_n, plane = GATED ? rank : 0;
-        for (int kb = 0; kb < p.blocks_k; ++kb, ++it) {
+        for (int kb = 0; kb < p.blocks_k; kb += kTileBlocks, ++it) {
           const int s = it % kTileStages;
           if (it >= kTileStages &&
               !warp_agrees(mbar_wait_cluster(empty + 8 * s, ((it / kTileStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty))) {
@@ -396,10 +401,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
           // the leader's barrier counts the bytes of both CTAs: this CTA's copies may land
           // there before the leader expects them, the phase still ends with its arrival
           const uint32_t bar = cluster_map(full + 8 * s, 0);
+          const int blocks = min(kTileBlocks, p.blocks_k - kb);
           if (elect_one()) {
-            if (rank == 0) mbar_expect_tx(full + 8 * s, stage_tx);
-            tma_pair_load_2d(stage, &p.x_map, kb * kBlockK, t0, bar);
-            tma_pair_load_3d(stage + kBoxBytes, &p.w_map, kb * kBlockK, row, plane, bar);
+            if (rank == 0) mbar_expect_tx(full + 8 * s, blocks * block_tx);
+            for (int j = 0; j < blocks; ++j) {
+              tma_pair_load_2d(stage + 2 * j * kBoxBytes, &p.x_map, (kb + j) * kBlockK, t0, bar);
+              tma_pair_load_3d(stage + (2 * j + 1) * kBoxBytes, &p.w_map, (kb + j) * kBlockK, row, plane, bar);
+            }
           }
           __syncwarp();
         }
@@ -419,7 +427,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
         const int b = n & 1;
         if (n >= 2 && !warp_agrees(mbar_wait_cluster(acc_empty + 8 * b, ((n >> 1) - 1) & 1, &g_int8_error, kErrTimeoutAcc))) break;
         tc_fence_after();
-        for (int kb = 0; kb < p.blocks_k; ++kb, ++it) {
+        for (int kb = 0; kb < p.blocks_k; kb += kTileBlocks, ++it) {
           const int s = it % kTileStages;
           if (!warp_agrees(mbar_wait_cluster(full + 8 * s, (it / kTileStages) & 1, &g_int8_error, kErrTimeoutFull))) {
             ok = false;
@@ -427,11 +435,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
           }
           tc_fence_after();
           const uint32_t stage = ring + s * kTileStageBytes;
-          const uint64_t x = smem_desc(stage, 16, 1024, kLayoutSw128);
-          const uint64_t w = smem_desc(stage + kBoxBytes, 16, 1024, kLayoutSw128);
+          const int blocks = min(kTileBlocks, p.blocks_k - kb);
           if (elect_one()) {
+            for (int j = 0; j < blocks; ++j) {
+              const uint64_t x = smem_desc(stage + 2 * j * kBoxBytes, 16, 1024, kLayoutSw128);
+              const uint64_t w = smem_desc(stage + (2 * j + 1) * kBoxBytes, 16, 1024, kLayoutSw128);
 #pragma unroll
-            for (int k = 0; k < kBlockK / 32; ++k) tc_pair_mma_i8(tmem + b * kTileN, x + 2 * k, w + 2 * k, idesc, kb > 0 || k > 0);
+              for (int k = 0; k < kBlockK / 32; ++k)
+                tc_pair_mma_i8(tmem + b * kTileN, x + 2 * k, w + 2 * k, idesc, kb > 0 || j > 0 || k > 0);
+            }
             tc_pair_commit(empty + 8 * s);
           }
           __syncwarp();
@@ -718,13 +730,16 @@ int run(const char *what, const Product &q, void *stream) {
   cudaError_t e;
   const int pairs = q.tokens > kTileTokens ? sm_pairs() : 0;
   if (pairs > 0) {
-    // the width that leaves the pairs the least to do, an epilogue counted as 32 columns
+    // the width that leaves the pairs the least to do: a tile's time grows as its width plus
+    // 192 columns (8192 x 7168 x 7168, a tile's share of the whole: 19.4 us at 256 columns,
+    // 13.0 at 128, 11.1 at 64). 2048 tokens: 224 columns 72 us, 256 columns 74, 128 columns 87;
+    // 1024 x 2048 x 7168: 128 columns 16.1 us, 256 columns 23.1.
     int64_t best = INT64_MAX;
     a.token_tiles = (q.tokens + kTileM - 1) / kTileM;
     for (int n = kTileN; n >= 64; n -= q.gated ? 64 : 32) {
       const int f = q.gated ? n / 2 : n;
       const int64_t tiles = static_cast<int64_t>(a.token_tiles) * ((q.features + f - 1) / f);
-      const int64_t cost = (tiles + pairs - 1) / pairs * (n + 32);
+      const int64_t cost = (tiles + pairs - 1) / pairs * (n + 192);
       if (cost < best) best = cost, a.tile_n = n, a.feature_tiles = (q.features + f - 1) / f;
     }
     const int es = q.out_type == MM_DTYPE_FP32 ? 4 : 2;
