@@ -12,11 +12,15 @@
 // rounded first because it is the stream that the next layers add to, and the norm reads
 // what they read (the rule of the peer hop in mm_comm.cu).
 //
-// Bound: memory. One CTA holds one row in registers (NV chunks of 16 bytes a thread), so
-// that x and the residual are read once and every output is written once. Few rows take
-// as many threads as the row has chunks (latency: one load a thread); many rows take 256
-// to 512 threads, so that several rows share an SM and one row's loads hide another's
-// reduction.
+// Bound: memory, and next to it the instructions of an element. norm_rows_kernel: one CTA
+// holds one row in registers, packed as it is stored (NV chunks of 16 bytes a thread), so
+// that x and the residual are read once, all their loads are in flight at once, and every
+// output is written once; 16-bit pairs are added packed (one rounding, the same as of the
+// fp32 sum: where that sum is inexact it is nowhere near a tie) and the fp32 arithmetic
+// goes by pairs (f32x2). Few rows take as many threads as the row has chunks (latency: one
+// load a thread); many rows take fewer, so that several rows share an SM and one row's
+// loads hide another's reduction. norm_kernel: rows that are too long to hold, or whose
+// buffers do not share an alignment, read again in each pass.
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -119,20 +123,7 @@ __device__ __forceinline__ void load_gamma(const NormArgs &a, int e0, float (&g)
   }
 }
 
-// Block-wide sum / maximum; every thread gets the result. `red` holds 32 words, and a
-// caller that reduces twice gives each its own.
-__device__ __forceinline__ float block_sum(float v, float *red) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  const int warps = blockDim.x >> 5;
-  if (warps == 1) return v;
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = (threadIdx.x & 31) < warps ? red[threadIdx.x & 31] : 0.0f;
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
+// Block-wide maximum; every thread gets the result.
 __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *red) {
   v = __reduce_max_sync(0xffffffffu, v);
   const int warps = blockDim.x >> 5;
@@ -162,13 +153,353 @@ __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, ui
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// One CTA per row. NV > 0: the row's chunks stay in registers (NV a thread). NV == 0: a row
-// too long for that, or rows whose buffers do not share an alignment (VEC == 1), is read
-// again from memory in each of the passes.
-template <typename T, int VEC, int NV, int QUANT>
+// ---------------------------------------------------------------------------------------
+// Packed arithmetic: a chunk is 16 bytes, VEC elements.
+struct alignas(8) F2 {
+  float x, y;
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 d;
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmul.rn.f32x2 r, p, q;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 d;
+  asm("{\n\t.reg .b64 p, q, r, s;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tmov.b64 r, {%6, %7};\n\t"
+      "fma.rn.f32x2 s, p, q, r;\n\tmov.b64 {%0, %1}, s;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 d;
+  asm("{\n\t.reg .b64 p, q, r;\n\tmov.b64 p, {%2, %3};\n\tmov.b64 q, {%4, %5};\n\tadd.rn.f32x2 r, p, q;\n\t"
+      "mov.b64 {%0, %1}, r;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
+template <typename T>
+struct Pack;  // of one 32-bit word
+template <>
+struct Pack<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ F2 value(uint32_t w) { return {__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)}; }
+  static __device__ __forceinline__ uint32_t round(F2 v) {
+    uint32_t d;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(v.y), "f"(v.x));
+    return d;
+  }
+};
+template <>
+struct Pack<__half> {
+  static __device__ __forceinline__ uint32_t add(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+  }
+  static __device__ __forceinline__ F2 value(uint32_t w) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+    return {f.x, f.y};
+  }
+  static __device__ __forceinline__ uint32_t round(F2 v) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(v.y), "f"(v.x));
+    return d;
+  }
+};
+
+// The words of a chunk as pairs of fp32 values and back.
+template <typename T>
+struct Chunk {
+  static constexpr int kVec = 16 / sizeof(T), kPairs = kVec / 2;
+  static __device__ __forceinline__ void values(const uint4 &q, F2 (&f)[kPairs]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (sizeof(T) == 4) {
+      f[0] = {__uint_as_float(w[0]), __uint_as_float(w[1])};
+      f[1] = {__uint_as_float(w[2]), __uint_as_float(w[3])};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[i] = Pack<T>::value(w[i]);
+    }
+  }
+  static __device__ __forceinline__ uint4 round(const F2 (&f)[kPairs]) {
+    if constexpr (sizeof(T) == 4)
+      return make_uint4(__float_as_uint(f[0].x), __float_as_uint(f[0].y), __float_as_uint(f[1].x), __float_as_uint(f[1].y));
+    else
+      return make_uint4(Pack<T>::round(f[0]), Pack<T>::round(f[1]), Pack<T>::round(f[2]), Pack<T>::round(f[3]));
+  }
+  static __device__ __forceinline__ uint4 add(const uint4 &a, const uint4 &b) {
+    if constexpr (sizeof(T) == 4)
+      return make_uint4(__float_as_uint(__fadd_rn(__uint_as_float(a.x), __uint_as_float(b.x))),
+                        __float_as_uint(__fadd_rn(__uint_as_float(a.y), __uint_as_float(b.y))),
+                        __float_as_uint(__fadd_rn(__uint_as_float(a.z), __uint_as_float(b.z))),
+                        __float_as_uint(__fadd_rn(__uint_as_float(a.w), __uint_as_float(b.w))));
+    else
+      return make_uint4(Pack<T>::add(a.x, b.x), Pack<T>::add(a.y, b.y), Pack<T>::add(a.z, b.z), Pack<T>::add(a.w, b.w));
+  }
+  // [e0, e0 + VEC) of a row of n; elements outside read as zero and are not written
+  static __device__ __forceinline__ uint4 load(const T *row, int e0, int n, bool whole) {
+    if (whole) return *reinterpret_cast<const uint4 *>(row + e0);
+    union { uint4 q; T t[kVec]; } u;
+    u.q = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (e0 + i >= 0 && e0 + i < n) u.t[i] = row[e0 + i];
+    return u.q;
+  }
+  static __device__ __forceinline__ void store(T *row, int e0, int n, bool whole, const uint4 &q) {
+    if (whole) {
+      *reinterpret_cast<uint4 *>(row + e0) = q;
+      return;
+    }
+    union { uint4 q; T t[kVec]; } u;
+    u.q = q;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i)
+      if (e0 + i >= 0 && e0 + i < n) row[e0 + i] = u.t[i];
+  }
+};
+
+// mx_scale_code, branch-free: the exponent of amax * fp32(1 / 448), rounded up when the
+// mantissa is not zero (a subnormal product rounds at 2^-127, its midpoint); a zero block
+// has scale 1, NaN and infinity code 255.
+__device__ __forceinline__ uint32_t mx_code(uint32_t amax_bits) {
+  const uint32_t b = __float_as_uint(__fmul_rn(__uint_as_float(amax_bits), 0x1.24924ap-9f));
+  const uint32_t c = (b + (b < 0x800000u ? 0x3fffffu : 0x7fffffu)) >> 23;
+  return amax_bits == 0u ? 127u : min(c, 255u);
+}
+
+// 1 / sqrt(sum / n + eps): the sum's last steps and Newton's step in 64 bits, so that one
+// rounding is left in the factor that a whole row shares.
+__device__ __forceinline__ float inverse_rms(double sum, int n, float eps) {
+  const double m = sum / n + static_cast<double>(eps);
+  const float y0 = rsqrtf(static_cast<float>(m));
+  if (!(y0 > 0.0f && y0 < __uint_as_float(0x7f800000u))) return y0;  // 0, inf, NaN
+  const double y = y0;
+  return static_cast<float>(y * (1.5 - 0.5 * m * y * y));
+}
+
+// Block-wide sum, and the maximum of `top` beside it.
+__device__ __forceinline__ double block_sum(double v, uint32_t &top, double *red, uint32_t *red_top) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  top = __reduce_max_sync(0xffffffffu, top);
+  const int warps = blockDim.x >> 5, lane = threadIdx.x & 31;
+  if (warps == 1) return v;
+  if (lane == 0) {
+    red[threadIdx.x >> 5] = v;
+    red_top[threadIdx.x >> 5] = top;
+  }
+  __syncthreads();
+  v = lane < warps ? red[lane] : 0.0;
+  top = __reduce_max_sync(0xffffffffu, lane < warps ? red_top[lane] : 0u);
+#pragma unroll
+  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// One CTA per row, NV chunks of it a thread, held in registers. Four and more take more than
+// the 64 registers that 1024 threads leave each.
+constexpr int row_threads(int nv, bool norm) { return nv >= 8 && norm ? 512 : nv >= 4 ? 640 : 1024; }
+template <typename T, int NV, int QUANT, bool NORM>
+__global__ void __launch_bounds__(row_threads(NV, NORM)) norm_rows_kernel(const __grid_constant__ NormArgs a) {
+  using C = Chunk<T>;
+  constexpr int VEC = C::kVec, PAIRS = C::kPairs;
+  __shared__ double red_d[32];
+  __shared__ uint32_t red_u[32], red_v[32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t t = blockIdx.x;
+  const int n = a.hidden;
+  const T *x = static_cast<const T *>(a.x) + t * a.ld_x;
+  const T *res = NORM && a.residual ? static_cast<const T *>(a.residual) + t * a.ld_residual : nullptr;
+  T *res_out = NORM && a.residual ? static_cast<T *>(a.residual_out) + t * a.ld_residual_out : nullptr;
+  T *norm = NORM && a.norm_out ? static_cast<T *>(a.norm_out) + t * a.ld_norm : nullptr;
+  uint8_t *codes = QUANT ? a.codes + t * a.ld_codes : nullptr;
+  // chunk c holds elements [c * VEC - shift, ...): chunks start on 16-byte boundaries of x,
+  // and of every other buffer of x's type (the host checked that they share the offset)
+  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  const int first = static_cast<int>(threadIdx.x) * VEC - shift, step = static_cast<int>(blockDim.x) * VEC;
+  auto whole = [&](int e0) { return e0 >= 0 && e0 + VEC <= n; };
+
+  uint4 v[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int e0 = first + j * step;
+    v[j] = e0 < n ? C::load(x, e0, n, whole(e0)) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  if (res) {
+    uint4 q[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = first + j * step;
+      q[j] = e0 < n ? C::load(res, e0, n, whole(e0)) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = first + j * step;
+      v[j] = C::add(v[j], q[j]);
+      if (e0 < n) C::store(res_out, e0, n, whole(e0), v[j]);
+    }
+  }
+
+  // gamma's values of chunk j; zero outside the row
+  auto gammas = [&](int j, float (&g)[VEC]) {
+    const int e0 = first + j * step;
+    if (e0 < n) {
+      load_gamma<T, VEC>(a, e0, g);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) g[i] = 0.0f;
+    }
+  };
+
+  F2 inv = {1.0f, 1.0f};
+  uint32_t top = 0u;
+  if constexpr (NORM) {
+    // a chain of NV * PAIRS terms a half, then 64 bits. int8: the largest |r gamma| on the way,
+    // so that one reduction gives both the factor and the scale
+    F2 ss = {0.0f, 0.0f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      F2 f[PAIRS];
+      C::values(v[j], f);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) ss = fma2(f[i], f[i], ss);
+      if constexpr (QUANT == MM_QUANT_INT8) {
+        float g[VEC];
+        gammas(j, g);
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          const F2 p = mul2(f[i], {g[2 * i], g[2 * i + 1]});
+          top = max(top, max(__float_as_uint(p.x) & 0x7fffffffu, __float_as_uint(p.y) & 0x7fffffffu));
+        }
+      }
+    }
+    const double sum = block_sum(static_cast<double>(ss.x) + static_cast<double>(ss.y), top, red_d, red_u);
+    inv.x = inv.y = inverse_rms(sum, n, a.eps);
+  }
+
+  // y of chunk j
+  auto scaled = [&](int j, F2 (&f)[PAIRS]) {
+    C::values(v[j], f);
+    if constexpr (NORM) {
+      float g[VEC];
+      gammas(j, g);
+#pragma unroll
+      for (int i = 0; i < PAIRS; ++i) f[i] = mul2(mul2(f[i], inv), {g[2 * i], g[2 * i + 1]});
+    }
+  };
+
+  if constexpr (QUANT != MM_QUANT_INT8) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = first + j * step;
+      F2 f[PAIRS];
+      scaled(j, f);
+      if (norm && e0 < n) C::store(norm, e0, n, whole(e0), C::round(f));
+      if constexpr (QUANT == MM_QUANT_MXFP8) {
+        // 32 / VEC neighbouring lanes share a block (H is a multiple of 32 and shift is 0 here)
+        uint32_t m = 0u;
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i)
+          m = max(m, max(__float_as_uint(f[i].x) & 0x7fffffffu, __float_as_uint(f[i].y) & 0x7fffffffu));
+#pragma unroll
+        for (int o = 16 / VEC; o; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const uint32_t code = mx_code(m);
+        const float by1 = mx_inverse(code);
+        const F2 by = {by1, by1};
+        if (e0 < n) {
+          uint32_t w[VEC / 4];
+#pragma unroll
+          for (int i = 0; i < VEC / 4; ++i) {
+            const F2 p = mul2(f[2 * i], by), q = mul2(f[2 * i + 1], by);
+            w[i] = e4m3x2(p.x, p.y) | static_cast<uint32_t>(e4m3x2(q.x, q.y)) << 16;
+          }
+          if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(codes + e0) = make_uint2(w[0], w[VEC / 4 - 1]);
+          else *reinterpret_cast<uint32_t *>(codes + e0) = w[0];
+          if (e0 % 32 == 0) static_cast<uint8_t *>(a.scales)[t * (n / 32) + e0 / 32] = static_cast<uint8_t>(code);
+        }
+      }
+    }
+  } else {
+    if constexpr (NORM) {
+      // max |r gamma| * inv is max |y| but for the order of two roundings (the quotient of the
+      // largest still rounds to 127), unless a product left the normal range
+      const bool normal = top >= 0x21800000u && top < 0x7b800000u && inv.x > 0x1p-60f && inv.x < 0x1p+60f;  // 2^-60, 2^120
+      if (normal) {
+        top = __float_as_uint(__fmul_rn(__uint_as_float(top), inv.x));
+      } else {
+        top = 0u;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          const int e0 = first + j * step;
+          F2 f[PAIRS];
+          scaled(j, f);
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (e0 + i >= 0 && e0 + i < n) top = max(top, __float_as_uint(i & 1 ? f[i / 2].y : f[i / 2].x) & 0x7fffffffu);
+        }
+        top = block_max(top, red_v);
+      }
+    } else {
+      // rows as they are: the packed halves' magnitudes
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (sizeof(T) == 4) top = max(top, w[i] & 0x7fffffffu);
+          else top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+        }
+      }
+      if constexpr (sizeof(T) == 2) top = __float_as_uint(Pack<T>::value(max(top & 0xffffu, top >> 16)).x);
+      top = block_max(top, red_u);
+    }
+    const bool finite = top < 0x7f800000u;
+    const float s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __uint_as_float(0x7fc00000u);
+    if (threadIdx.x == 0) static_cast<float *>(a.scales)[t] = s;
+    const bool tiny = !(s >= 0x1p-120f);  // s = 0 and NaN too
+    const float r = tiny ? 0.0f : __fdiv_rn(1.0f, s);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = first + j * step;
+      if (e0 >= n) continue;
+      F2 f[PAIRS];
+      scaled(j, f);
+      if (norm) C::store(norm, e0, n, whole(e0), C::round(f));
+      uint32_t q[VEC];
+      if (tiny) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) q[i] = finite ? int8_code_tiny(i & 1 ? f[i / 2].y : f[i / 2].x, s) : 0u;
+      } else {
+        const F2 r2 = {r, r}, s2 = {-s, -s}, magic = {0x1.8p+23f, 0x1.8p+23f};
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {  // int8_code, by pairs
+          const F2 d = mul2(f[i], r2);
+          const F2 k = add2(fma2(fma2(d, s2, f[i]), r2, d), magic);
+          q[2 * i] = __float_as_uint(k.x);
+          q[2 * i + 1] = __float_as_uint(k.y);
+        }
+      }
+      uint32_t w[VEC / 4];
+#pragma unroll
+      for (int i = 0; i < VEC / 4; ++i) w[i] = pack4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
+      store_codes<VEC>(codes, e0, n, w, a.codes_wide && shift == 0 && e0 + VEC <= n);
+    }
+  }
+}
+
+// One CTA per row, read again from memory in each of the passes: rows too long for registers,
+// or (VEC == 1) rows whose buffers do not share an alignment.
+template <typename T, int VEC, int QUANT>
 __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float red_f[32];
-  __shared__ uint32_t red_u[32];
+  __shared__ double red_d[32];
+  __shared__ uint32_t red_u[32], red_v[32];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t t = blockIdx.x;
@@ -182,8 +513,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
   // and of every other buffer of x's type (the host checked that they share the offset)
   const int shift = VEC > 1 ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : 0;
   const int chunks = (n + shift + VEC - 1) / VEC;
-  constexpr int HOLD = NV ? NV : 1;
-  float v[HOLD][VEC];
+  float v[VEC];
 
   // r of chunk c (c < chunks)
   auto fetch = [&](int c, float (&out)[VEC]) {
@@ -202,42 +532,17 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
 
   float inv = 1.0f;
   if (a.gamma) {
-    float ss = 0.0f;
-    if constexpr (NV > 0) {
+    // a chain of a few terms a thread at a time, then 64 bits: rows of any length
+    double sum = 0.0;
+    for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
+      fetch(c, v);
+      float ss = 0.0f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = threadIdx.x + j * blockDim.x;
-        if (c < chunks) {
-          fetch(c, v[j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) v[j][i] = 0.0f;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) ss = __fmaf_rn(v[j][i], v[j][i], ss);
-    } else {
-      for (int c = threadIdx.x; c < chunks; c += blockDim.x) {
-        fetch(c, v[0]);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) ss = __fmaf_rn(v[0][i], v[0][i], ss);
-      }
+      for (int i = 0; i < VEC; ++i) ss = __fmaf_rn(v[i], v[i], ss);
+      sum += static_cast<double>(ss);
     }
-    ss = block_sum(ss, red_f);
-    inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(n)), a.eps)));
-  } else if constexpr (NV > 0) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = threadIdx.x + j * blockDim.x;
-      if (c < chunks) {
-        fetch(c, v[j]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[j][i] = 0.0f;
-      }
-    }
+    uint32_t none = 0u;
+    inv = inverse_rms(block_sum(sum, none, red_d, red_u), n, a.eps);
   }
 
   // y of chunk c from its r
@@ -294,74 +599,68 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
 
   // every lane of a warp walks the same number of chunks: the block maxima shuffle
   const int rounds = (chunks + blockDim.x - 1) / blockDim.x;
-  if constexpr (NV > 0) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int c = threadIdx.x + j * blockDim.x;
-      if (c < chunks) {
-        keep(c, v[j]);
-        scale(c, v[j]);
-        if (norm) store_chunk<T, VEC>(norm, c * VEC - shift, n, v[j]);
-      }
-      if constexpr (QUANT == MM_QUANT_MXFP8) mx_block(c, v[j]);
-      if constexpr (QUANT == MM_QUANT_INT8) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
-      }
-    }
-  } else {
+  {
     for (int j = 0; j < rounds; ++j) {
       const int c = threadIdx.x + j * blockDim.x;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[0][i] = 0.0f;
+      for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
       if (c < chunks) {
-        fetch(c, v[0]);
-        if constexpr (QUANT != MM_QUANT_INT8) keep(c, v[0]);
-        scale(c, v[0]);
-        if (norm) store_chunk<T, VEC>(norm, c * VEC - shift, n, v[0]);
+        fetch(c, v);
+        if constexpr (QUANT != MM_QUANT_INT8) keep(c, v);
+        scale(c, v);
+        if (norm) store_chunk<T, VEC>(norm, c * VEC - shift, n, v);
       }
-      if constexpr (QUANT == MM_QUANT_MXFP8) mx_block(c, v[0]);
+      if constexpr (QUANT == MM_QUANT_MXFP8) mx_block(c, v);
       if constexpr (QUANT == MM_QUANT_INT8) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(v[0][i]) & 0x7fffffffu);
+        for (int i = 0; i < VEC; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
       }
     }
   }
 
   if constexpr (QUANT == MM_QUANT_INT8) {
-    top = block_max(top, red_u);
+    top = block_max(top, red_v);
     const bool finite = top < 0x7f800000u;
     const float s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __uint_as_float(0x7fc00000u);
     if (threadIdx.x == 0) static_cast<float *>(a.scales)[t] = s;
     const bool tiny = !(s >= 0x1p-120f);  // s = 0 and NaN too
     const float r = tiny ? 0.0f : __fdiv_rn(1.0f, s);
-    if constexpr (NV > 0) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int c = threadIdx.x + j * blockDim.x;
-        if (c < chunks) {
-          if (!finite) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[j][i] = 0.0f;
-          }
-          int8_chunk(c, v[j], finite ? s : 0.0f, r, tiny);
-        }
-      }
-    } else {
+    {
       for (int j = 0; j < rounds; ++j) {
         const int c = threadIdx.x + j * blockDim.x;
         if (c < chunks) {
-          fetch(c, v[0]);
-          keep(c, v[0]);
-          scale(c, v[0]);
+          fetch(c, v);
+          keep(c, v);
+          scale(c, v);
           if (!finite) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[0][i] = 0.0f;
+            for (int i = 0; i < VEC; ++i) v[i] = 0.0f;
           }
-          int8_chunk(c, v[0], finite ? s : 0.0f, r, tiny);
+          int8_chunk(c, v, finite ? s : 0.0f, r, tiny);
         }
       }
     }
+  }
+}
+
+// Chunks a thread. Few rows: as few as its threads allow (one row's latency). Many rows: more,
+// so that more loads of more rows are in flight; measured (bf16, us): norm + MXFP8 of 8192 x
+// 7168: two 98, four 83 (6.4 TB/s), eight 101; of 4096 x 16384: four 94, eight 128; of 8192 x
+// 2048: one 28, two 26; of 1024 x 5120: two 8.3, four 10.5, eight 16.8. int8 rows alone hold
+// less beside the row: 4096 x 16384: four 42, eight 35; 8192 x 7168: two 41, four 33, eight 30.5.
+template <typename T, int QUANT, bool NORM>
+cudaError_t launch_rows(const NormArgs &a, int chunks, void *stream) {
+  const unsigned rows = static_cast<unsigned>(a.tokens);
+  auto threads = [&](int nv) { return dim3(((chunks + nv - 1) / nv + 31) / 32 * 32); };
+  int nv;
+  if (a.tokens <= kFewRows) nv = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
+  else if (!NORM) nv = chunks <= 256 ? 2 : chunks <= 512 ? 4 : 8;
+  else nv = chunks <= (a.tokens <= 2048 ? 1024 : 512) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
+  switch (nv) {
+    case 1: return launch(norm_rows_kernel<T, 1, QUANT, NORM>, dim3(rows), threads(1), 0, stream, a);
+    case 2: return launch(norm_rows_kernel<T, 2, QUANT, NORM>, dim3(rows), threads(2), 0, stream, a);
+    case 4: return launch(norm_rows_kernel<T, 4, QUANT, NORM>, dim3(rows), threads(4), 0, stream, a);
+    default: return launch(norm_rows_kernel<T, 8, QUANT, NORM>, dim3(rows), threads(8), 0, stream, a);
   }
 }
 
@@ -369,20 +668,15 @@ template <typename T, int QUANT>
 cudaError_t launch_norm(const NormArgs &a, bool wide, void *stream) {
   constexpr int VEC = 16 / sizeof(T);
   const unsigned rows = static_cast<unsigned>(a.tokens);
-  auto up32 = [](int v) { return (v + 31) / 32 * 32; };
-  if (!wide) return launch(norm_kernel<T, 1, 0, QUANT>, dim3(rows), dim3(std::min(1024, up32(a.hidden))), 0, stream, a);
+  if (!wide)
+    return launch(norm_kernel<T, 1, QUANT>, dim3(rows), dim3(std::min(1024, (a.hidden + 31) / 32 * 32)), 0, stream, a);
   // one chunk more than the row fills where rows start inside a 16-byte unit
   const bool shifted = (reinterpret_cast<uintptr_t>(a.x) % 16) || (a.ld_x * static_cast<int64_t>(sizeof(T))) % 16;
   const int chunks = (a.hidden + VEC - 1) / VEC + (shifted ? 1 : 0);
-  if (a.tokens <= kFewRows) {
-    const int threads = std::min(1024, up32(chunks));
-    const int nv = (chunks + threads - 1) / threads;
-    if (nv == 1) return launch(norm_kernel<T, VEC, 1, QUANT>, dim3(rows), dim3(threads), 0, stream, a);
-    if (nv == 2) return launch(norm_kernel<T, VEC, 2, QUANT>, dim3(rows), dim3(up32((chunks + 1) / 2)), 0, stream, a);
-  }
-  if (chunks <= 512) return launch(norm_kernel<T, VEC, 2, QUANT>, dim3(rows), dim3(up32((chunks + 1) / 2)), 0, stream, a);
-  if (chunks <= 4096) return launch(norm_kernel<T, VEC, 4, QUANT>, dim3(rows), dim3(up32((chunks + 3) / 4)), 0, stream, a);
-  return launch(norm_kernel<T, VEC, 0, QUANT>, dim3(rows), dim3(1024), 0, stream, a);
+  if (chunks > 8 * row_threads(8, a.gamma != nullptr)) return launch(norm_kernel<T, VEC, QUANT>, dim3(rows), dim3(1024), 0, stream, a);
+  if constexpr (QUANT == MM_QUANT_INT8)
+    if (!a.gamma) return launch_rows<T, QUANT, false>(a, chunks, stream);
+  return launch_rows<T, QUANT, true>(a, chunks, stream);
 }
 
 template <typename T>
