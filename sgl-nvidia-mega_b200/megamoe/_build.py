@@ -1,4 +1,5 @@
-"""In-tree build of libmegamoe.so for sm_100a (nvcc cross-compiles without a GPU).
+"""In-tree build of libmegamoe.so for sm_100a (nvcc cross-compiles without a GPU), and
+of _dense.so, the dense operators' calls on torch tensors (host code over the C ABI).
 
 Each translation unit compiles to its own object (in parallel), then one link:
 mm_gate_dsv41.cu takes the DeepSeek-V4.1 gate's floating-point flags
@@ -20,9 +21,12 @@ CSRC = os.path.join(PKG, "csrc")
 SOURCES = ["mm_api.cu", "mm_route.cu", "mm_gate_dsv41.cu", "mm_experts.cu", "mm_finalize.cu", "mm_comm.cu", "mm_norm.cu",
            "mm_int8.cu"]
 HEADERS = ["mm_dense.cuh", "mm_gate.cuh", "mm_kernels.cuh", "mm_layout.cuh", "mm_numerics.cuh", "mm_ptx.cuh"]
+TORCH_SOURCE = "mm_dense_torch.cpp"
 OUTPUT = os.path.join(HERE, "libmegamoe.so")
+TORCH_OUTPUT = os.path.join(HERE, "_dense.so")
 OBJDIR = os.path.join(HERE, "_build")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
+CXX = os.environ.get("CXX", "g++")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMPILE = [*ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC"]
 # per-file floating-point flags (the DeepSeek-V4.1 gate's, routed_expert_gemm.py:213-220)
@@ -34,14 +38,39 @@ def compile_flags(source: str) -> list:
     return [*COMPILE, *FILE_FLAGS.get(source, []), "-I", os.path.join(REPO, "include"), "-I", CSRC]
 
 
+def torch_command() -> list:
+    """g++ command that builds _dense.so against the running Python and torch."""
+    import sysconfig
+
+    import torch
+
+    root = os.path.dirname(torch.__file__)
+    lib = os.path.join(root, "lib")
+    abi = int(torch.compiled_with_cxx11_abi())
+    includes = [os.path.join(REPO, "include"), sysconfig.get_paths()["include"], os.path.join(root, "include"),
+                os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    return [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *(f"-I{i}" for i in includes),
+            os.path.join(CSRC, TORCH_SOURCE), "-o", TORCH_OUTPUT, f"-L{HERE}", "-l:libmegamoe.so", "-Wl,-rpath,$ORIGIN",
+            f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+            f"-Wl,-rpath,{lib}",
+            # the C++ runtime that torch runs on: a toolchain with a static one alone would put
+            # a second copy, and a second set of stream locales, beside it
+            "-nostdlib++", "-l:libstdc++.so.6"]
+
+
+def _older(output: str, deps) -> bool:
+    return not os.path.exists(output) or any(os.path.getmtime(p) > os.path.getmtime(output) for p in deps)
+
+
 def _stale() -> bool:
-    if not os.path.exists(OUTPUT):
-        return True
-    built = os.path.getmtime(OUTPUT)
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(REPO, "include", "megamoe.h"))
-    deps.append(os.path.abspath(__file__))
-    return any(os.path.getmtime(p) > built for p in deps)
+    own = [os.path.join(REPO, "include", "megamoe.h"), os.path.abspath(__file__)]
+    return _older(OUTPUT, [os.path.join(CSRC, f) for f in SOURCES + HEADERS] + own) or _torch_stale()
+
+
+def _torch_stale() -> bool:
+    return _older(TORCH_OUTPUT, [os.path.join(CSRC, TORCH_SOURCE), os.path.join(REPO, "include", "megamoe.h"),
+                                 os.path.abspath(__file__)])
 
 
 def _run(cmd, verbose):
@@ -70,6 +99,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError(f"nvcc link failed ({res.returncode}) building {OUTPUT}")
+    if force or _torch_stale():
+        cmd = torch_command()
+        res = _run(cmd, verbose)
+        if res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+            raise RuntimeError(f"g++ failed ({res.returncode}): {' '.join(cmd)}")
     return OUTPUT
 
 
