@@ -26,6 +26,31 @@ struct NormArgs {
   int codes_wide;            // code rows start on 8-byte boundaries
 };
 
+// The code rint(y / s), in the low byte. y / s by y * r, r = 1 / s, and one correction from the
+// exact remainder (Markstein's division: two fused operations instead of a full divide);
+// adding 1.5 * 2^23 rounds to the nearest even integer and leaves it, in two's complement,
+// in the low byte. |y| <= amax keeps the quotient within 127 after rounding.
+__device__ __forceinline__ uint32_t int8_code(float y, float s, float r) {
+  const float q = __fmul_rn(y, r);
+  const float t = __fmaf_rn(__fmaf_rn(-q, s, y), r, q);
+  return __float_as_uint(__fadd_rn(t, 0x1.8p+23f));
+}
+// The same below the range in which 1 / s is finite: a true divide, clamped because a
+// subnormal s carries few bits (the quotient may pass 127).
+__device__ __forceinline__ uint32_t int8_code_tiny(float y, float s) {
+  const float t = s == 0.0f ? 0.0f : __fdiv_rn(y, s);
+  return __float_as_uint(__fadd_rn(fminf(fmaxf(t, -127.0f), 127.0f), 0x1.8p+23f));
+}
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// The scale of a row whose largest magnitude has these bits: NaN unless it is finite.
+__device__ __forceinline__ float int8_scale(uint32_t top) {
+  return top < 0x7f800000u ? __fdiv_rn(__uint_as_float(top), 127.0f) : __uint_as_float(0x7fc00000u);
+}
+// Scales below this (zero and NaN too) take int8_code_tiny.
+constexpr float kTinyScale = 0x1p-120f;
+
 // int8 codes and fp32 scales of rows (mm_norm.cu); returns an MM_* status.
 int quantize_rows(const char *what, const void *x, int64_t ld_x, int dtype, int8_t *codes, int64_t ld_codes,
                   float *scales, int tokens, int hidden, void *stream);

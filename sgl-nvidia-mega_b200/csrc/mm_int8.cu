@@ -39,7 +39,7 @@ constexpr int kRowsM = 128;           // weight rows of a box, token rows of a p
 constexpr int kBoxBytes = kRowsM * kBlockK;
 
 // Above this many tokens the tile form takes over.
-constexpr int kTileTokens = 256;
+constexpr int kTileTokens = 128;
 
 // Error word of this file's launches: bounded waits that ran out (mm_int8_check).
 __device__ uint32_t g_int8_error;
@@ -59,6 +59,10 @@ struct alignas(64) Int8Args {
   int has_clamp;
   float clamp;
   int token_tiles, feature_tiles, tile_n;  // of the tile form
+  const float *h;       // [tokens, ld_h] fp32, the operand of the requantizing form
+  int64_t ld_h;
+  uint32_t *tile_max;   // [tokens, tiles of h] largest |h| (bits) of each gated tile
+  int h_tiles;
   int split;            // CTAs of a cluster that share a tile's depth (stream form)
 };
 
@@ -106,9 +110,18 @@ __device__ __forceinline__ void store4(const Int8Args &p, int64_t at, int left, 
 // ---------------------------------------------------------------------------------------
 // The stream form. Two CTAs share an SM (at most 113 KB each), so that one's start, its
 // accumulator read and its reduction run under the other's loads.
-template <int BN, bool GATED>
+enum : int {
+  kLinear,   // x's codes by TMA, out by scales and bias
+  kGated,    // gate and up rows, out h = silu(gate) * up
+  kRequant,  // x's codes made here from h: the down product of few tokens. The row's scale comes
+             // from the maxima that the gated tiles left, so no launch stands between the two
+             // products (a row kernel there costs about 2 us of a 16 us block)
+};
+constexpr int kRequantTokens = 16;
+
+template <int BN, int KIND>
 struct Stream {
-  static constexpr int kA = GATED ? 2 : 1;
+  static constexpr int kA = KIND == kGated ? 2 : 1;
   static constexpr int kStageBytes = kA * kBoxBytes + BN * kBlockK;
   static constexpr int kRing = 108 * 1024;
   static constexpr int kStages = kRing / kStageBytes;
@@ -123,10 +136,12 @@ struct Stream {
 constexpr int kStreamThreads = 192;
 constexpr int kStreamWarps = kStreamThreads / 32;
 
-template <int BN, bool GATED>
+template <int BN, int KIND>
 __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __grid_constant__ Int8Args p) {
-  using S = Stream<BN, GATED>;
+  using S = Stream<BN, KIND>;
+  constexpr bool GATED = KIND == kGated;
   extern __shared__ uint8_t smem_raw[];
+  __shared__ float row_scale[kRequantTokens], row_inverse[kRequantTokens];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t ring = (raw + 1023u) & ~1023u;
   uint8_t *ring_ptr = smem_raw + (ring - raw);
@@ -152,7 +167,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
 #pragma unroll
       for (int a = 0; a < S::kA; ++a) tma_prefetch_3d(&p.w_map, (kb0 + i) * kBlockK, f0, a);
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(full + 8 * s, 1);
+      mbar_init(full + 8 * s, KIND == kRequant ? 5 : 1);  // the loads, and four warps' codes
       mbar_init(empty + 8 * s, 1);
     }
     mbar_init(acc, 1);
@@ -167,13 +182,19 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *slot_ptr;
-  // only now: a dependent's CTA that started sooner could take the TMEM columns that a CTA
-  // of this launch on the same SM still waits for, and then wait for this launch to end
-  pdl_launch_dependents();
+  // Dependents start only now. After the allocation: a dependent's CTA that started sooner
+  // could take the TMEM columns that a CTA of this launch on the same SM still waits for, and
+  // then wait for this launch to end. After the wait: whatever ran before this launch's
+  // predecessor has ended by then. So in the requantizing form, whose predecessor is the gated
+  // product, w2 is no longer being written when this launch starts, and its loads need not
+  // wait; in the others the predecessor may be what wrote the weights.
+  if (KIND != kRequant || warp != 0) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
 
   if (warp == 0) {
     {
-      pdl_wait();
       const uint64_t stream_once = policy_evict_first(), keep = policy_evict_last();
       int i = 0;
       for (; i < n; ++i) {
@@ -184,11 +205,11 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
         const uint32_t stage = ring + s * S::kStageBytes;
         const int k = (kb0 + i) * kBlockK;
         if (elect_one()) {
-          mbar_expect_tx(full + 8 * s, S::kStageBytes);
+          mbar_expect_tx(full + 8 * s, KIND == kRequant ? S::kA * kBoxBytes : S::kStageBytes);
 #pragma unroll
           for (int a = 0; a < S::kA; ++a)
             tma_load_3d(stage + a * kBoxBytes, &p.w_map, k, f0, a, full + 8 * s, gridDim.y > 1 ? keep : stream_once);
-          tma_load_2d(stage + S::kA * kBoxBytes, &p.x_map, k, t0, full + 8 * s, keep);
+          if (KIND != kRequant) tma_load_2d(stage + S::kA * kBoxBytes, &p.x_map, k, t0, full + 8 * s, keep);
         }
         __syncwarp();
       }
@@ -225,11 +246,73 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       mbar_wait_drain(acc, 0);
     }
     __syncwarp();
+  } else if constexpr (KIND == kRequant) {
+    // Warps 2..5 make the tokens' codes: token t by warp 2 + t % 4, four depths a lane, one stage
+    // ahead in registers. (Depths past h's width meet weights that TMA filled with zero.)
+    constexpr int kEach = kRequantTokens / 4;
+    const int w = warp - 2;
+    float4 next[kEach];
+    auto fetch = [&](int i) {
+      const int64_t k = static_cast<int64_t>(kb0 + i) * kBlockK + 4 * lane;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int t = w + 4 * e;
+        next[e] = t < p.tokens && k < p.ld_h ? __ldcg(reinterpret_cast<const float4 *>(p.h + t * p.ld_h + k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+    };
+    fetch(0);
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int t = w + 4 * e;
+      if (t >= p.tokens) continue;
+      uint32_t top = 0u;
+      for (int i = lane; i < p.h_tiles; i += 32) top = max(top, __ldcg(p.tile_max + static_cast<int64_t>(t) * p.h_tiles + i));
+      top = __reduce_max_sync(0xffffffffu, top);
+      const float s = int8_scale(top);
+      if (lane == 0) {
+        row_scale[t] = s;
+        row_inverse[t] = s >= kTinyScale ? __fdiv_rn(1.0f, s) : 0.0f;
+      }
+    }
+    __syncwarp();
+    for (int i = 0; i < n; ++i) {
+      const int s = i % S::kStages;
+      float4 v[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) v[e] = next[e];
+      if (i + 1 < n) fetch(i + 1);
+      if (i >= S::kStages &&
+          !warp_agrees(mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty)))
+        break;
+      uint8_t *codes = ring_ptr + s * S::kStageBytes + S::kA * kBoxBytes;
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int t = w + 4 * e;
+        if (t >= p.tokens) continue;
+        const float rs = row_scale[t], ri = row_inverse[t];
+        uint32_t word;
+        if (rs >= kTinyScale)
+          word = pack4(int8_code(v[e].x, rs, ri), int8_code(v[e].y, rs, ri), int8_code(v[e].z, rs, ri), int8_code(v[e].w, rs, ri));
+        else if (rs == rs)
+          word = pack4(int8_code_tiny(v[e].x, rs), int8_code_tiny(v[e].y, rs), int8_code_tiny(v[e].z, rs), int8_code_tiny(v[e].w, rs));
+        else
+          word = 0u;
+        // as TMA would place it: 16-byte units XORed with the row
+        *reinterpret_cast<uint32_t *>(codes + t * kBlockK + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = word;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full + 8 * s);
+    }
+    __syncwarp();
   }
 
   // Every warp takes part in the reduction; warps 2..5 first bring the sums from TMEM (warp w
   // reads lanes 32 (w % 4) and on: weight rows) into the ring's place, token-major.
-  pdl_wait();
+  if (KIND == kRequant && warp == 0) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
   const int live = min(BN, p.tokens - t0);
   const int width = p.out_type == MM_DTYPE_FP32 ? 16 : 8;
   const int es = p.out_type == MM_DTYPE_FP32 ? 4 : 2;
@@ -283,7 +366,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
         }
       }
       const int t = t0 + c0 + j;
-      const float xs = p.x_scale[t];
+      const float xs = KIND == kRequant ? row_scale[t] : p.x_scale[t];
       float v[4];
       const int s0[4] = {sum[0].x, sum[0].y, sum[0].z, sum[0].w};
       if constexpr (GATED) {
@@ -297,6 +380,14 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
         for (int i = 0; i < 4; ++i) v[i] = __fmaf_rn(__fmul_rn(static_cast<float>(s0[i]), xs), ws[0][i], bias[i]);
       }
       if (ok && left > 0) store4(p, t * p.ld_out + f, left, v, wide);
+      if (GATED && p.tile_max != nullptr) {
+        uint32_t top = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i < left) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) p.tile_max[static_cast<int64_t>(t) * p.h_tiles + f0 / kRowsM] = top;
+      }
     }
     // the parts are read: the next chunk may take their place, or the CTA may end
     if (split > 1) cluster_sync();
@@ -622,18 +713,18 @@ cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, int clust
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <int BN, bool GATED>
+template <int BN, int KIND>
 cudaError_t launch_stream(Int8Args &a, void *stream) {
-  using S = Stream<BN, GATED>;
+  using S = Stream<BN, KIND>;
   static bool done[64] = {};
-  const cudaError_t e = raise_smem(int8_stream_kernel<BN, GATED>, S::kSmem, done);
+  const cudaError_t e = raise_smem(int8_stream_kernel<BN, KIND>, S::kSmem, done);
   if (e != cudaSuccess) return e;
   const int tiles = (a.features + kRowsM - 1) / kRowsM, token_tiles = (a.tokens + BN - 1) / BN;
   // enough CTAs for two an SM, each with at least two stages of depth
   int split = 1;
   while (split < 8 && static_cast<int64_t>(tiles) * token_tiles * split < 148 && 4 * split <= a.blocks_k) split *= 2;
   a.split = split;
-  return launch_cluster(int8_stream_kernel<BN, GATED>, dim3(tiles * split, token_tiles), kStreamThreads, S::kSmem, split, stream, a);
+  return launch_cluster(int8_stream_kernel<BN, KIND>, dim3(tiles * split, token_tiles), kStreamThreads, S::kSmem, split, stream, a);
 }
 
 // CTA pairs that the current device runs at once (of the tile form: one CTA an SM, all its
@@ -689,6 +780,9 @@ struct Product {
   int out_type, tokens, features, depth;  // gated: features of h, w holds twice as many rows
   bool gated;
   float clamp;
+  bool out_pad;         // the columns from features to ld_out may be written
+  uint32_t *tile_max;   // gated: [tokens, tiles] maxima out; else with h: the requantizing form
+  const float *h;       // in place of x and x_scale, rows ld_x values apart
 };
 
 int check(const char *what, const Product &q) {
@@ -700,7 +794,7 @@ int check(const char *what, const Product &q) {
   if (q.out_type != MM_DTYPE_BF16 && q.out_type != MM_DTYPE_FP16 && q.out_type != MM_DTYPE_FP32)
     return set_error(MM_ERR_INVALID, "%s: unknown output type %d", what, q.out_type);
   if (q.tokens == 0) return MM_OK;
-  if (!q.x || !q.x_scale || !q.w || !q.w_scale || !q.out) return set_error(MM_ERR_INVALID, "%s: null pointer", what);
+  if (!(q.h || (q.x && q.x_scale)) || !q.w || !q.w_scale || !q.out) return set_error(MM_ERR_INVALID, "%s: null pointer", what);
   if (q.ld_x < q.depth || q.ld_w < q.depth || q.ld_out < q.features)
     return set_error(MM_ERR_INVALID, "%s: a row stride below the row's length", what);
   if (!aligned(q.x, 16) || !aligned(q.w, 16) || q.ld_x % 16 || q.ld_w % 16)
@@ -724,6 +818,10 @@ int run(const char *what, const Product &q, void *stream) {
   a.gated = q.gated;
   a.has_clamp = q.clamp > 0.0f;
   a.clamp = q.clamp;
+  a.h = q.h;
+  a.ld_h = q.ld_x;
+  a.tile_max = q.tile_max;
+  a.h_tiles = ((q.gated ? q.features : q.depth) + kRowsM - 1) / kRowsM;
   auto w_map = [&](int rows) { return encode(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, q.depth, q.features, q.gated ? 2 : 1, q.ld_w, rows); };
   int rc;
   auto x_map = [&](int rows) { return encode(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, q.depth, q.tokens, 0, q.ld_x, rows); };
@@ -743,7 +841,7 @@ int run(const char *what, const Product &q, void *stream) {
       if (cost < best) best = cost, a.tile_n = n, a.feature_tiles = (q.features + f - 1) / f;
     }
     const int es = q.out_type == MM_DTYPE_FP32 ? 4 : 2;
-    a.stage_out = aligned(q.out, 16) && q.ld_out * es % 16 == 0 && static_cast<int64_t>(q.features) * es % 16 == 0;
+    a.stage_out = aligned(q.out, 16) && q.ld_out * es % 16 == 0 && (q.out_pad || static_cast<int64_t>(q.features) * es % 16 == 0);
     if ((rc = x_map(kRowsM)) || (rc = w_map(a.tile_n / 2))) return rc;
     if (a.stage_out &&
         (rc = encode(&a.out_map, q.out_type == MM_DTYPE_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
@@ -759,20 +857,24 @@ int run(const char *what, const Product &q, void *stream) {
     return MM_OK;
   }
   if ((rc = w_map(kRowsM))) return rc;
+  if (q.h) {
+    if ((e = launch_stream<16, kRequant>(a, stream)) != cudaSuccess) return set_error(MM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
+    return MM_OK;
+  }
   const int most = q.gated ? 128 : 256;
   int bn = 16;
   while (bn < q.tokens && bn < most) bn *= 2;
   if ((rc = x_map(bn))) return rc;
   switch (q.gated ? -bn : bn) {
-    case 16: e = launch_stream<16, false>(a, stream); break;
-    case 32: e = launch_stream<32, false>(a, stream); break;
-    case 64: e = launch_stream<64, false>(a, stream); break;
-    case 128: e = launch_stream<128, false>(a, stream); break;
-    case 256: e = launch_stream<256, false>(a, stream); break;
-    case -16: e = launch_stream<16, true>(a, stream); break;
-    case -32: e = launch_stream<32, true>(a, stream); break;
-    case -64: e = launch_stream<64, true>(a, stream); break;
-    default: e = launch_stream<128, true>(a, stream); break;
+    case 16: e = launch_stream<16, kLinear>(a, stream); break;
+    case 32: e = launch_stream<32, kLinear>(a, stream); break;
+    case 64: e = launch_stream<64, kLinear>(a, stream); break;
+    case 128: e = launch_stream<128, kLinear>(a, stream); break;
+    case 256: e = launch_stream<256, kLinear>(a, stream); break;
+    case -16: e = launch_stream<16, kGated>(a, stream); break;
+    case -32: e = launch_stream<32, kGated>(a, stream); break;
+    case -64: e = launch_stream<64, kGated>(a, stream); break;
+    default: e = launch_stream<128, kGated>(a, stream); break;
   }
   if (e != cudaSuccess) return set_error(MM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return MM_OK;
@@ -790,7 +892,7 @@ extern "C" {
 int mm_int8_linear(const int8_t *x, int64_t ld_x, const float *x_scale, const int8_t *w, int64_t ld_w,
                    const float *w_scale, const float *bias, void *out, int64_t ld_out, int32_t out_dtype,
                    int32_t tokens, int32_t features, int32_t depth, void *stream) {
-  const Product q = {x, ld_x, x_scale, w, ld_w, w_scale, bias, out, ld_out, out_dtype, tokens, features, depth, false, 0.0f};
+  const Product q = {x, ld_x, x_scale, w, ld_w, w_scale, bias, out, ld_out, out_dtype, tokens, features, depth, false, 0.0f, false, nullptr, nullptr};
   const int rc = check("mm_int8_linear", q);
   if (rc || tokens == 0) return rc;
   return run("mm_int8_linear", q, stream);
@@ -798,7 +900,7 @@ int mm_int8_linear(const int8_t *x, int64_t ld_x, const float *x_scale, const in
 
 int64_t mm_int8_ffn_workspace(int32_t tokens, int32_t inter) {
   if (tokens < 1 || inter < 1) return 0;
-  return up(static_cast<int64_t>(tokens) * inter * 4, 256) + up(tokens * up(inter, 16), 256) + static_cast<int64_t>(tokens) * 4;
+  return up(tokens * up(inter, 4) * 4, 256) + up(tokens * up(inter, 16), 256) + static_cast<int64_t>(tokens) * 4;
 }
 
 int mm_int8_ffn(const mm_int8_ffn_args *f, void *stream) {
@@ -810,20 +912,29 @@ int mm_int8_ffn(const mm_int8_ffn_args *f, void *stream) {
   if (f->tokens > 0 && (!ws || !aligned(ws, 256) || f->workspace_bytes < mm_int8_ffn_workspace(f->tokens, f->inter)))
     return set_error(MM_ERR_INVALID, "mm_int8_ffn: the workspace needs %lld bytes on a 256-byte boundary",
                      static_cast<long long>(mm_int8_ffn_workspace(f->tokens, f->inter)));
-  // h in fp32 (its rounding to int8 is the only one), then its codes and scales
-  const int64_t ld_q = up(f->inter, 16);
+  // h in fp32 (its rounding to int8 is the only one), rows on 16-byte boundaries; then its codes
+  // and scales, or few tokens' tile maxima in their place
+  const int64_t ld_h = up(f->inter, 4), ld_q = up(f->inter, 16);
   float *h = reinterpret_cast<float *>(ws);
-  int8_t *hq = ws ? reinterpret_cast<int8_t *>(ws + up(static_cast<int64_t>(f->tokens) * f->inter * 4, 256)) : nullptr;
+  int8_t *hq = ws ? reinterpret_cast<int8_t *>(ws + up(f->tokens * ld_h * 4, 256)) : nullptr;
   float *hs = ws ? reinterpret_cast<float *>(hq + up(f->tokens * ld_q, 256)) : nullptr;
-  const Product up_q = {f->x, f->ld_x, f->x_scale, f->w13, f->ld_w13, f->w13_scale, nullptr, h, f->inter, MM_DTYPE_FP32,
-                        f->tokens, f->inter, f->hidden, true, f->clamp};
-  const Product down_q = {hq, ld_q, hs, f->w2, f->ld_w2, f->w2_scale, nullptr, f->out, f->ld_out, f->out_dtype,
-                          f->tokens, f->hidden, f->inter, false, 0.0f};
+  const bool few = f->tokens <= kRequantTokens;
+  const Product up_q = {f->x, f->ld_x, f->x_scale, f->w13, f->ld_w13, f->w13_scale, nullptr, h, ld_h, MM_DTYPE_FP32,
+                        f->tokens, f->inter, f->hidden, true, f->clamp, true,
+                        few ? reinterpret_cast<uint32_t *>(hq) : nullptr, nullptr};
+  Product down_q = {hq, ld_q, hs, f->w2, f->ld_w2, f->w2_scale, nullptr, f->out, f->ld_out, f->out_dtype,
+                    f->tokens, f->hidden, f->inter, false, 0.0f, false, nullptr, nullptr};
   int rc = check("mm_int8_ffn", up_q);
   if (!rc) rc = check("mm_int8_ffn", down_q);
   if (rc || f->tokens == 0) return rc;
   if ((rc = run("mm_int8_ffn", up_q, stream))) return rc;
-  if ((rc = quantize_rows("mm_int8_ffn", h, f->inter, MM_DTYPE_FP32, hq, ld_q, hs, f->tokens, f->inter, stream))) return rc;
+  if (few) {
+    down_q.h = h;
+    down_q.ld_x = ld_h;
+    down_q.tile_max = up_q.tile_max;
+  } else if ((rc = quantize_rows("mm_int8_ffn", h, ld_h, MM_DTYPE_FP32, hq, ld_q, hs, f->tokens, f->inter, stream))) {
+    return rc;
+  }
   return run("mm_int8_ffn", down_q, stream);
 }
 

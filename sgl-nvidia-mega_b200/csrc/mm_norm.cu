@@ -134,25 +134,6 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t *red) {
   return __reduce_max_sync(0xffffffffu, v);
 }
 
-// Four codes rint(y / s) in a word. y / s by y * r, r = 1 / s, and one correction from the
-// exact remainder (Markstein's division: two fused operations instead of a full divide);
-// adding 1.5 * 2^23 rounds to the nearest even integer and leaves it, in two's complement,
-// in the low byte. |y| <= amax keeps the quotient within 127 after rounding.
-__device__ __forceinline__ uint32_t int8_code(float y, float s, float r) {
-  const float q = __fmul_rn(y, r);
-  const float t = __fmaf_rn(__fmaf_rn(-q, s, y), r, q);
-  return __float_as_uint(__fadd_rn(t, 0x1.8p+23f));
-}
-// The same below the range in which 1 / s is finite: a true divide, clamped because a
-// subnormal s carries few bits (the quotient may pass 127).
-__device__ __forceinline__ uint32_t int8_code_tiny(float y, float s) {
-  const float t = s == 0.0f ? 0.0f : __fdiv_rn(y, s);
-  return __float_as_uint(__fadd_rn(fminf(fmaxf(t, -127.0f), 127.0f), 0x1.8p+23f));
-}
-__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
-
 // ---------------------------------------------------------------------------------------
 // Packed arithmetic: a chunk is 16 bytes, VEC elements.
 struct alignas(8) F2 {
@@ -461,9 +442,9 @@ __global__ void __launch_bounds__(row_threads(NV, NORM)) norm_rows_kernel(const 
       top = block_max(top, red_u);
     }
     const bool finite = top < 0x7f800000u;
-    const float s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __uint_as_float(0x7fc00000u);
+    const float s = int8_scale(top);
     if (threadIdx.x == 0) static_cast<float *>(a.scales)[t] = s;
-    const bool tiny = !(s >= 0x1p-120f);  // s = 0 and NaN too
+    const bool tiny = !(s >= kTinyScale);
     const float r = tiny ? 0.0f : __fdiv_rn(1.0f, s);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
@@ -621,9 +602,9 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
   if constexpr (QUANT == MM_QUANT_INT8) {
     top = block_max(top, red_v);
     const bool finite = top < 0x7f800000u;
-    const float s = finite ? __fdiv_rn(__uint_as_float(top), 127.0f) : __uint_as_float(0x7fc00000u);
+    const float s = int8_scale(top);
     if (threadIdx.x == 0) static_cast<float *>(a.scales)[t] = s;
-    const bool tiny = !(s >= 0x1p-120f);  // s = 0 and NaN too
+    const bool tiny = !(s >= kTinyScale);
     const float r = tiny ? 0.0f : __fdiv_rn(1.0f, s);
     {
       for (int j = 0; j < rounds; ++j) {

@@ -344,6 +344,46 @@ def test_rows_do_not_depend_on_their_batch(tokens):
         assert torch.equal(whole[t:t + 1], megamoe.int8_linear(int8_rows(x[t:t + 1]), xs[t:t + 1], w, ws))
 
 
+@pytest.mark.parametrize("hidden,inter", [(512, 1990), (1000, 77), (256, 4096)])
+def test_ffn_rows_do_not_depend_on_their_batch(hidden, inter):
+    """One token, the largest batch that makes h's codes inside the down product, the first that
+    makes them in a launch of their own, and many tokens: the same bits a row."""
+    g = gen(hidden, inter, 4)
+    x, xs = weights(300, hidden, g)
+    w13, s13 = weights(2 * inter, hidden, g)
+    w2, s2 = weights(hidden, inter, g)
+    xs = xs * math.sqrt(hidden)
+    whole = megamoe.int8_ffn(x, xs, w13, s13, w2, s2, clamp=3.0)
+    for t in (1, 5, 16, 17, 64, 65, 128, 129):
+        assert torch.equal(whole[:t], megamoe.int8_ffn(x[:t], xs[:t], w13, s13, w2, s2, clamp=3.0)), t
+
+
+def test_weights_written_just_before_the_call():
+    """The launches start early and fetch weights early: never before they are written."""
+    g = gen(12)
+    w13a, s13 = weights(2 * 2048, 1024, g)
+    w2a, s2 = weights(1024, 2048, g)
+    w13b, w2b = w13a.flip(0).contiguous(), w2a.flip(0).contiguous()
+    x, xs = weights(4, 1024, g)
+    want = [megamoe.int8_ffn(x, xs, a, s13, b, s2) for a, b in ((w13a, w2a), (w13b, w2b))]
+    w13, w2 = w13a.clone(), w2a.clone()
+    got = []
+    for k in range(40):
+        w13.copy_(w13b if k % 2 else w13a)
+        w2.copy_(w2b if k % 2 else w2a)
+        got.append(megamoe.int8_ffn(x, xs, w13, s13, w2, s2))
+    for k, y in enumerate(got):
+        assert torch.equal(y, want[k % 2]), k
+    # and by an operator of this library that lets its successor start early
+    f = randn((4096, 1024), g)
+    for k in range(20):
+        f.mul_(-1)
+        q, qs = megamoe.quantize_int8(f)
+        y = megamoe.int8_linear(x, xs, q, qs)
+        torch.cuda.synchronize()
+        assert torch.equal(y, megamoe.int8_linear(x, xs, q, qs)), k
+
+
 def test_empty_batches():
     e = torch.empty
     x = e((0, 64), dtype=torch.int8, device="cuda")
