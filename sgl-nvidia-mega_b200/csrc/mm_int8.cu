@@ -9,7 +9,7 @@
 // tcgen05 kind::i8, operands by TMA as 128-byte-swizzled K-major boxes of 128 bytes of depth.
 // Two forms:
 //  * int8_stream_kernel (few tokens; bound by the weights' stream). 128 weight rows are the
-//    MMA's M side and up to 256 tokens its N side, so one token costs one column and the
+//    MMA's M side and up to 128 tokens its N side, so one token costs one column and the
 //    tokens' padding costs no memory traffic. Few tiles do not fill the GPU: the CTAs of a
 //    cluster share a tile's depth, and add their integer parts through distributed shared
 //    memory, each finishing its share of the tokens. No workspace, no atomics, no counters.
@@ -17,8 +17,9 @@
 //    256 weight rows (cta_group::2: each CTA stages half of either operand, half the shared
 //    memory traffic of two single tiles), persistent, with two accumulators in TMEM so that
 //    the epilogue of one tile runs under the products of the next.
-// A gated tile takes 128 gate rows and the 128 up rows of the same features into two halves
-// of the accumulator: gate and up of one element sit in the same TMEM lane.
+// A gated tile takes gate rows and the up rows of the same features together: 64 and 64 as the
+// 128 rows of the stream form (they meet in shared memory, where its parts are added anyway),
+// 128 and 128 as the two halves of the tile form's columns (one TMEM lane then holds both).
 #include <algorithm>
 #include <cstdint>
 #include <cuda.h>
@@ -79,29 +80,33 @@ __device__ __forceinline__ float gate_up(const Int8Args &p, float g, float u) {
   return __fmul_rn(u, __fdiv_rn(g, __fadd_rn(1.0f, expf(-g))));
 }
 
-// Four consecutive features of one token.
-__device__ __forceinline__ void store4(const Int8Args &p, int64_t at, int left, const float (&v)[4], bool wide) {
+// PER (two or four) consecutive features of one token, `left` of them inside the row.
+template <int PER>
+__device__ __forceinline__ void store_some(const Int8Args &p, int64_t at, int left, const float (&v)[PER], bool wide) {
   if (p.out_type == MM_DTYPE_FP32) {
     float *o = static_cast<float *>(p.out) + at;
-    if (wide && left >= 4) {
-      *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
+    if (wide && left >= PER) {
+      if constexpr (PER == 4) *reinterpret_cast<float4 *>(o) = make_float4(v[0], v[1], v[2], v[3]);
+      else *reinterpret_cast<float2 *>(o) = make_float2(v[0], v[1]);
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < PER; ++i)
         if (i < left) o[i] = v[i];
     }
   } else {
-    uint16_t h[4];
+    uint16_t h[PER];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < PER; ++i)
       h[i] = p.out_type == MM_DTYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v[i]))
                                          : __half_as_ushort(__float2half_rn(v[i]));
     uint16_t *o = static_cast<uint16_t *>(p.out) + at;
-    if (wide && left >= 4) {
-      *reinterpret_cast<uint2 *>(o) = make_uint2(h[0] | static_cast<uint32_t>(h[1]) << 16, h[2] | static_cast<uint32_t>(h[3]) << 16);
+    if (wide && left >= PER) {
+      const uint32_t lo = h[0] | static_cast<uint32_t>(h[1]) << 16;
+      if constexpr (PER == 4) *reinterpret_cast<uint2 *>(o) = make_uint2(lo, h[2] | static_cast<uint32_t>(h[3]) << 16);
+      else *reinterpret_cast<uint32_t *>(o) = lo;
     } else {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < PER; ++i)
         if (i < left) o[i] = h[i];
     }
   }
@@ -121,16 +126,14 @@ constexpr int kRequantTokens = 16;
 
 template <int BN, int KIND>
 struct Stream {
-  static constexpr int kA = KIND == kGated ? 2 : 1;
-  static constexpr int kStageBytes = kA * kBoxBytes + BN * kBlockK;
+  static constexpr int kFeatures = KIND == kGated ? kRowsM / 2 : kRowsM;  // of a tile
+  static constexpr int kStageBytes = kBoxBytes + BN * kBlockK;
   static constexpr int kRing = 108 * 1024;
   static constexpr int kStages = kRing / kStageBytes;
-  // tokens whose parts are staged at once: 64 KB at most, in the ring's place
-  static constexpr int kChunk = BN < 128 / kA ? BN : 128 / kA;
-  static constexpr int kCols = kA * BN < 32 ? 32 : kA * BN;  // TMEM columns, a power of two
+  static constexpr int kCols = BN < 32 ? 32 : BN;  // TMEM columns, a power of two
   static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
   static_assert(kStages >= 2 && kCols <= 256, "two CTAs an SM share 512 columns");
-  static_assert(kChunk * kA * 512 <= kStages * kStageBytes, "parts fit the ring");
+  static_assert(BN * kRowsM * 4 <= kStages * kStageBytes, "the parts take the ring's place");
 };
 
 constexpr int kStreamThreads = 192;
@@ -153,8 +156,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = p.split;
   const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
-  const int f0 = (blockIdx.x / split) * kRowsM;
-  const int t0 = blockIdx.y * BN;
+  const int f0 = (blockIdx.x / split) * S::kFeatures;
   const int kb0 = p.blocks_k * rank / split, kb1 = p.blocks_k * (rank + 1) / split;
   const int n = kb1 - kb0;
 
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
 #pragma unroll 1
     for (int i = 0; i < n && i < S::kStages; ++i)
 #pragma unroll
-      for (int a = 0; a < S::kA; ++a) tma_prefetch_3d(&p.w_map, (kb0 + i) * kBlockK, f0, a);
+      for (int a = 0; a < kRowsM / S::kFeatures; ++a) tma_prefetch_3d(&p.w_map, (kb0 + i) * kBlockK, f0, a);
     for (int s = 0; s < S::kStages; ++s) {
       mbar_init(full + 8 * s, KIND == kRequant ? 5 : 1);  // the loads, and four warps' codes
       mbar_init(empty + 8 * s, 1);
@@ -205,11 +207,11 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
         const uint32_t stage = ring + s * S::kStageBytes;
         const int k = (kb0 + i) * kBlockK;
         if (elect_one()) {
-          mbar_expect_tx(full + 8 * s, KIND == kRequant ? S::kA * kBoxBytes : S::kStageBytes);
+          mbar_expect_tx(full + 8 * s, KIND == kRequant ? kBoxBytes : S::kStageBytes);
 #pragma unroll
-          for (int a = 0; a < S::kA; ++a)
-            tma_load_3d(stage + a * kBoxBytes, &p.w_map, k, f0, a, full + 8 * s, gridDim.y > 1 ? keep : stream_once);
-          if (KIND != kRequant) tma_load_2d(stage + S::kA * kBoxBytes, &p.x_map, k, t0, full + 8 * s, keep);
+          for (int a = 0; a < kRowsM / S::kFeatures; ++a)
+            tma_load_3d(stage + a * S::kFeatures * kBlockK, &p.w_map, k, f0, a, full + 8 * s, stream_once);
+          if (KIND != kRequant) tma_load_2d(stage + kBoxBytes, &p.x_map, k, 0, full + 8 * s, keep);
         }
         __syncwarp();
       }
@@ -228,15 +230,12 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
         }
         tc_fence_after();
         const uint32_t stage = ring + s * S::kStageBytes;
-        const uint64_t b = smem_desc(stage + S::kA * kBoxBytes, 16, 1024, kLayoutSw128);
+        const uint64_t w = smem_desc(stage, 16, 1024, kLayoutSw128);
+        const uint64_t b = smem_desc(stage + kBoxBytes, 16, 1024, kLayoutSw128);
         if (elect_one()) {
 #pragma unroll
-          for (int a = 0; a < S::kA; ++a) {
-            const uint64_t w = smem_desc(stage + a * kBoxBytes, 16, 1024, kLayoutSw128);
-#pragma unroll
-            for (int k = 0; k < kBlockK / 32; ++k)  // 32 bytes of depth an instruction
-              tc_mma_i8(tmem + a * BN, w + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
-          }
+          for (int k = 0; k < kBlockK / 32; ++k)  // 32 bytes of depth an instruction
+            tc_mma_i8(tmem, w + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
           tc_commit(empty + 8 * s);
         }
         __syncwarp();
@@ -261,17 +260,17 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       }
     };
     fetch(0);
+    uint32_t top[kEach] = {};
+    for (int i = lane; i < p.h_tiles; i += 32)
+#pragma unroll
+      for (int e = 0; e < kEach; ++e)
+        if (w + 4 * e < p.tokens) top[e] = max(top[e], __ldcg(p.tile_max + static_cast<int64_t>(w + 4 * e) * p.h_tiles + i));
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int t = w + 4 * e;
-      if (t >= p.tokens) continue;
-      uint32_t top = 0u;
-      for (int i = lane; i < p.h_tiles; i += 32) top = max(top, __ldcg(p.tile_max + static_cast<int64_t>(t) * p.h_tiles + i));
-      top = __reduce_max_sync(0xffffffffu, top);
-      const float s = int8_scale(top);
+      const float s = int8_scale(__reduce_max_sync(0xffffffffu, top[e]));
       if (lane == 0) {
-        row_scale[t] = s;
-        row_inverse[t] = s >= kTinyScale ? __fdiv_rn(1.0f, s) : 0.0f;
+        row_scale[w + 4 * e] = s;
+        row_inverse[w + 4 * e] = s >= kTinyScale ? __fdiv_rn(1.0f, s) : 0.0f;
       }
     }
     __syncwarp();
@@ -284,7 +283,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       if (i >= S::kStages &&
           !warp_agrees(mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty)))
         break;
-      uint8_t *codes = ring_ptr + s * S::kStageBytes + S::kA * kBoxBytes;
+      uint8_t *codes = ring_ptr + s * S::kStageBytes + kBoxBytes;
 #pragma unroll
       for (int e = 0; e < kEach; ++e) {
         const int t = w + 4 * e;
@@ -313,86 +312,74 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     pdl_wait();
     pdl_launch_dependents();
   }
-  const int live = min(BN, p.tokens - t0);
-  const int width = p.out_type == MM_DTYPE_FP32 ? 16 : 8;
+  // a lane finishes PER neighbouring features of a token
+  constexpr int PER = S::kFeatures / 32;
   const int es = p.out_type == MM_DTYPE_FP32 ? 4 : 2;
-  const bool wide = reinterpret_cast<uintptr_t>(p.out) % width == 0 && p.ld_out * es % width == 0;
-  const int f = f0 + 4 * lane;
+  const bool wide = reinterpret_cast<uintptr_t>(p.out) % (PER * es) == 0 && p.ld_out % PER == 0;
+  const int f = f0 + PER * lane;
   const int left = p.features - f;
-  float ws[S::kA][4], bias[4];
+  float ws[PER], second[PER];  // second: the bias, or the up rows' scales
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-#pragma unroll
-    for (int a = 0; a < S::kA; ++a) ws[a][i] = i < left ? p.w_scale[static_cast<int64_t>(a) * p.features + f + i] : 0.0f;
-    bias[i] = p.bias && i < left ? p.bias[f + i] : 0.0f;
+  for (int i = 0; i < PER; ++i) {
+    ws[i] = i < left ? p.w_scale[f + i] : 0.0f;
+    second[i] = i >= left ? 0.0f : GATED ? p.w_scale[static_cast<int64_t>(p.features) + f + i] : p.bias ? p.bias[f + i] : 0.0f;
   }
   bool ok = mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc);
   tc_fence_after();
   ok = ok && *failed == 0u;
-  for (int c0 = 0; c0 < live; c0 += S::kChunk) {
-    const int count = min(S::kChunk, live - c0);
-    if (warp >= 2) {
-      const int q = warp & 3;
+  if (warp >= 2) {
+    const int q = warp & 3;
 #pragma unroll 1
-      for (int j = 0; j < count; j += 16) {
+    for (int j = 0; j < p.tokens; j += 16) {
+      uint32_t r[16];
+      tc_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + j, r);
+      tc_wait_ld();
+      uint32_t *to = reinterpret_cast<uint32_t *>(ring_ptr) + j * kRowsM + q * 32 + lane;
 #pragma unroll
-        for (int a = 0; a < S::kA; ++a) {
-          uint32_t r[16];
-          tc_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + a * BN + c0 + j, r);
-          tc_wait_ld();
-          uint32_t *to = reinterpret_cast<uint32_t *>(ring_ptr) + (j * S::kA + a) * kRowsM + q * 32 + lane;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) to[i * S::kA * kRowsM] = r[i];
-        }
-      }
+      for (int i = 0; i < 16; ++i) to[i * kRowsM] = r[i];
     }
-    if (split > 1) cluster_sync();
-    else __syncthreads();
-#pragma unroll 1
-    for (int j = rank * kStreamWarps + warp; j < count; j += split * kStreamWarps) {
-      int4 sum[S::kA];
-#pragma unroll
-      for (int a = 0; a < S::kA; ++a) {
-        const uint32_t at = ring + ((j * S::kA + a) * kRowsM + 4 * lane) * 4;
-        if (split > 1) {
-          sum[a] = make_int4(0, 0, 0, 0);
-#pragma unroll 4
-          for (int r = 0; r < split; ++r) {
-            const int4 v = cluster_load_v4(cluster_map(at, r));
-            sum[a].x += v.x, sum[a].y += v.y, sum[a].z += v.z, sum[a].w += v.w;
-          }
-        } else {
-          sum[a] = *reinterpret_cast<const int4 *>(ring_ptr + (at - ring));
-        }
-      }
-      const int t = t0 + c0 + j;
-      const float xs = KIND == kRequant ? row_scale[t] : p.x_scale[t];
-      float v[4];
-      const int s0[4] = {sum[0].x, sum[0].y, sum[0].z, sum[0].w};
-      if constexpr (GATED) {
-        const int s1[4] = {sum[1].x, sum[1].y, sum[1].z, sum[1].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          v[i] = gate_up(p, __fmul_rn(__fmul_rn(static_cast<float>(s0[i]), xs), ws[0][i]),
-                         __fmul_rn(__fmul_rn(static_cast<float>(s1[i]), xs), ws[1][i]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __fmaf_rn(__fmul_rn(static_cast<float>(s0[i]), xs), ws[0][i], bias[i]);
-      }
-      if (ok && left > 0) store4(p, t * p.ld_out + f, left, v, wide);
-      if (GATED && p.tile_max != nullptr) {
-        uint32_t top = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (i < left) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) p.tile_max[static_cast<int64_t>(t) * p.h_tiles + f0 / kRowsM] = top;
-      }
-    }
-    // the parts are read: the next chunk may take their place, or the CTA may end
-    if (split > 1) cluster_sync();
-    else __syncthreads();
   }
+  if (split > 1) cluster_sync();
+  else __syncthreads();
+#pragma unroll 1
+  for (int j = rank * kStreamWarps + warp; j < p.tokens; j += split * kStreamWarps) {
+    // the parts of four sums: four features, or two features' gate and up
+    const uint32_t at = ring + (j * kRowsM + PER * lane) * 4;
+    int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int r = 0; r < split; ++r) {
+      const uint32_t from = cluster_map(at, r);
+      if constexpr (GATED) {
+        const int2 g = cluster_load_v2(from), u = cluster_load_v2(from + 4 * S::kFeatures);
+        sum.x += g.x, sum.y += g.y, sum.z += u.x, sum.w += u.y;
+      } else {
+        const int4 v = cluster_load_v4(from);
+        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+      }
+    }
+    const int64_t t = j;
+    const float xs = KIND == kRequant ? row_scale[t] : p.x_scale[t];
+    const float a[4] = {__fmul_rn(static_cast<float>(sum.x), xs), __fmul_rn(static_cast<float>(sum.y), xs),
+                        __fmul_rn(static_cast<float>(sum.z), xs), __fmul_rn(static_cast<float>(sum.w), xs)};
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if constexpr (GATED) v[i] = gate_up(p, __fmul_rn(a[i], ws[i]), __fmul_rn(a[PER + i], second[i]));
+      else v[i] = __fmaf_rn(a[i], ws[i], second[i]);
+    }
+    if (ok && left > 0) store_some<PER>(p, t * p.ld_out + f, left, v, wide);
+    if (GATED && p.tile_max != nullptr) {
+      uint32_t top = 0u;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (i < left) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) p.tile_max[static_cast<int64_t>(t) * p.h_tiles + f0 / S::kFeatures] = top;
+    }
+  }
+  // the parts are read: the CTA may end
+  if (split > 1) cluster_sync();
+  else __syncthreads();
   tc_fence_before();
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, S::kCols);
@@ -719,12 +706,12 @@ cudaError_t launch_stream(Int8Args &a, void *stream) {
   static bool done[64] = {};
   const cudaError_t e = raise_smem(int8_stream_kernel<BN, KIND>, S::kSmem, done);
   if (e != cudaSuccess) return e;
-  const int tiles = (a.features + kRowsM - 1) / kRowsM, token_tiles = (a.tokens + BN - 1) / BN;
+  const int tiles = (a.features + S::kFeatures - 1) / S::kFeatures;
   // enough CTAs for two an SM, each with at least two stages of depth
   int split = 1;
-  while (split < 8 && static_cast<int64_t>(tiles) * token_tiles * split < 148 && 4 * split <= a.blocks_k) split *= 2;
+  while (split < 8 && tiles * split < 148 && 4 * split <= a.blocks_k) split *= 2;
   a.split = split;
-  return launch_cluster(int8_stream_kernel<BN, KIND>, dim3(tiles * split, token_tiles), kStreamThreads, S::kSmem, split, stream, a);
+  return launch_cluster(int8_stream_kernel<BN, KIND>, dim3(tiles * split), kStreamThreads, S::kSmem, split, stream, a);
 }
 
 // CTA pairs that the current device runs at once (of the tile form: one CTA an SM, all its
@@ -821,13 +808,14 @@ int run(const char *what, const Product &q, void *stream) {
   a.h = q.h;
   a.ld_h = q.ld_x;
   a.tile_max = q.tile_max;
-  a.h_tiles = ((q.gated ? q.features : q.depth) + kRowsM - 1) / kRowsM;
+  a.h_tiles = ((q.gated ? q.features : q.depth) + kRowsM / 2 - 1) / (kRowsM / 2);
   auto w_map = [&](int rows) { return encode(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, q.depth, q.features, q.gated ? 2 : 1, q.ld_w, rows); };
   int rc;
   auto x_map = [&](int rows) { return encode(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, q.depth, q.tokens, 0, q.ld_x, rows); };
   cudaError_t e;
-  const int pairs = q.tokens > kTileTokens ? sm_pairs() : 0;
-  if (pairs > 0) {
+  if (q.tokens > kTileTokens) {
+    const int pairs = sm_pairs();
+    if (pairs < 1) return set_error(MM_ERR_CUDA, "%s: the tile form does not fit this device", what);
     // the width that leaves the pairs the least to do: a tile's time grows as its width plus
     // 192 columns (8192 x 7168 x 7168, a tile's share of the whole: 19.4 us at 256 columns,
     // 13.0 at 128, 11.1 at 64). 2048 tokens: 224 columns 72 us, 256 columns 74, 128 columns 87;
@@ -856,21 +844,19 @@ int run(const char *what, const Product &q, void *stream) {
     if (e != cudaSuccess) return set_error(MM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
     return MM_OK;
   }
-  if ((rc = w_map(kRowsM))) return rc;
+  if ((rc = w_map(q.gated ? kRowsM / 2 : kRowsM))) return rc;
   if (q.h) {
     if ((e = launch_stream<16, kRequant>(a, stream)) != cudaSuccess) return set_error(MM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
     return MM_OK;
   }
-  const int most = q.gated ? 128 : 256;
   int bn = 16;
-  while (bn < q.tokens && bn < most) bn *= 2;
+  while (bn < q.tokens) bn *= 2;
   if ((rc = x_map(bn))) return rc;
   switch (q.gated ? -bn : bn) {
     case 16: e = launch_stream<16, kLinear>(a, stream); break;
     case 32: e = launch_stream<32, kLinear>(a, stream); break;
     case 64: e = launch_stream<64, kLinear>(a, stream); break;
     case 128: e = launch_stream<128, kLinear>(a, stream); break;
-    case 256: e = launch_stream<256, kLinear>(a, stream); break;
     case -16: e = launch_stream<16, kGated>(a, stream); break;
     case -32: e = launch_stream<32, kGated>(a, stream); break;
     case -64: e = launch_stream<64, kGated>(a, stream); break;

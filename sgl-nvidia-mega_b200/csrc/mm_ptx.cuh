@@ -311,6 +311,11 @@ __device__ __forceinline__ int4 cluster_load_v4(uint32_t addr) {
                : "memory");
   return v;
 }
+__device__ __forceinline__ int2 cluster_load_v2(uint32_t addr) {
+  int2 v;
+  asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t mapped_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(mapped_bar)
                : "memory");
