@@ -60,10 +60,7 @@ struct alignas(64) Int8Args {
   int has_clamp;
   float clamp;
   int token_tiles, feature_tiles, tile_n;  // of the tile form
-  const float *h;       // [tokens, ld_h] fp32, the operand of the requantizing form
-  int64_t ld_h;
-  uint32_t *tile_max;   // [tokens, tiles of h] largest |h| (bits) of each gated tile
-  int h_tiles;
+  int w_early;          // the launch's predecessors do not write the weights: load before waiting
   int split;            // CTAs of a cluster that share a tile's depth (stream form)
 };
 
@@ -115,18 +112,9 @@ __device__ __forceinline__ void store_some(const Int8Args &p, int64_t at, int le
 // ---------------------------------------------------------------------------------------
 // The stream form. Two CTAs share an SM (at most 113 KB each), so that one's start, its
 // accumulator read and its reduction run under the other's loads.
-enum : int {
-  kLinear,   // x's codes by TMA, out by scales and bias
-  kGated,    // gate and up rows, out h = silu(gate) * up
-  kRequant,  // x's codes made here from h: the down product of few tokens. The row's scale comes
-             // from the maxima that the gated tiles left, so no launch stands between the two
-             // products (a row kernel there costs about 2 us of a 16 us block)
-};
-constexpr int kRequantTokens = 16;
-
-template <int BN, int KIND>
+template <int BN, bool GATED>
 struct Stream {
-  static constexpr int kFeatures = KIND == kGated ? kRowsM / 2 : kRowsM;  // of a tile
+  static constexpr int kFeatures = GATED ? kRowsM / 2 : kRowsM;  // of a tile
   static constexpr int kStageBytes = kBoxBytes + BN * kBlockK;
   static constexpr int kRing = 108 * 1024;
   static constexpr int kStages = kRing / kStageBytes;
@@ -139,12 +127,10 @@ struct Stream {
 constexpr int kStreamThreads = 192;
 constexpr int kStreamWarps = kStreamThreads / 32;
 
-template <int BN, int KIND>
+template <int BN, bool GATED>
 __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __grid_constant__ Int8Args p) {
-  using S = Stream<BN, KIND>;
-  constexpr bool GATED = KIND == kGated;
+  using S = Stream<BN, GATED>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ float row_scale[kRequantTokens], row_inverse[kRequantTokens];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t ring = (raw + 1023u) & ~1023u;
   uint8_t *ring_ptr = smem_raw + (ring - raw);
@@ -169,7 +155,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
 #pragma unroll
       for (int a = 0; a < kRowsM / S::kFeatures; ++a) tma_prefetch_3d(&p.w_map, (kb0 + i) * kBlockK, f0, a);
     for (int s = 0; s < S::kStages; ++s) {
-      mbar_init(full + 8 * s, KIND == kRequant ? 5 : 1);  // the loads, and four warps' codes
+      mbar_init(full + 8 * s, 1);
       mbar_init(empty + 8 * s, 1);
     }
     mbar_init(acc, 1);
@@ -187,131 +173,71 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   // Dependents start only now. After the allocation: a dependent's CTA that started sooner
   // could take the TMEM columns that a CTA of this launch on the same SM still waits for, and
   // then wait for this launch to end. After the wait: whatever ran before this launch's
-  // predecessor has ended by then. So in the requantizing form, whose predecessor is the gated
-  // product, w2 is no longer being written when this launch starts, and its loads need not
-  // wait; in the others the predecessor may be what wrote the weights.
-  if (KIND != kRequant || warp != 0) {
+  // predecessor has ended by then, so that a launch two further on, whose own predecessor is
+  // known not to write its weights, may load them at once (w_early).
+  if (warp != 0) {
     pdl_wait();
     pdl_launch_dependents();
   }
 
   if (warp == 0) {
-    {
-      const uint64_t stream_once = policy_evict_first(), keep = policy_evict_last();
-      int i = 0;
-      for (; i < n; ++i) {
-        const int s = i % S::kStages;
-        if (i >= S::kStages &&
-            !warp_agrees(mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty)))
-          break;
-        const uint32_t stage = ring + s * S::kStageBytes;
-        const int k = (kb0 + i) * kBlockK;
-        if (elect_one()) {
-          mbar_expect_tx(full + 8 * s, KIND == kRequant ? kBoxBytes : S::kStageBytes);
+    const uint64_t stream_once = policy_evict_first(), keep = policy_evict_last();
+    auto load_w = [&](int i) {
+      const uint32_t stage = ring + (i % S::kStages) * S::kStageBytes, bar = full + 8 * (i % S::kStages);
+      mbar_expect_tx(bar, S::kStageBytes);
 #pragma unroll
-          for (int a = 0; a < kRowsM / S::kFeatures; ++a)
-            tma_load_3d(stage + a * S::kFeatures * kBlockK, &p.w_map, k, f0, a, full + 8 * s, stream_once);
-          if (KIND != kRequant) tma_load_2d(stage + kBoxBytes, &p.x_map, k, 0, full + 8 * s, keep);
-        }
-        __syncwarp();
-      }
-      // leave no copy in flight, whatever ended the loop
-      for (int j = max(0, i - S::kStages); j < i; ++j) mbar_wait_drain(full + 8 * (j % S::kStages), (j / S::kStages) & 1);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    {
-      constexpr uint32_t idesc = idesc_i8(kRowsM, BN);
-      for (int i = 0; i < n; ++i) {
-        const int s = i % S::kStages;
-        if (!warp_agrees(mbar_wait(full + 8 * s, (i / S::kStages) & 1, &g_int8_error, kErrTimeoutFull))) {
-          *failed = 1u;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t stage = ring + s * S::kStageBytes;
-        const uint64_t w = smem_desc(stage, 16, 1024, kLayoutSw128);
-        const uint64_t b = smem_desc(stage + kBoxBytes, 16, 1024, kLayoutSw128);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < kBlockK / 32; ++k)  // 32 bytes of depth an instruction
-            tc_mma_i8(tmem, w + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
-          tc_commit(empty + 8 * s);
-        }
-        __syncwarp();
-      }
-      if (elect_one()) tc_commit(acc);
-      __syncwarp();
-      mbar_wait_drain(acc, 0);
-    }
-    __syncwarp();
-  } else if constexpr (KIND == kRequant) {
-    // Warps 2..5 make the tokens' codes: token t by warp 2 + t % 4, four depths a lane, one stage
-    // ahead in registers. (Depths past h's width meet weights that TMA filled with zero.)
-    constexpr int kEach = kRequantTokens / 4;
-    const int w = warp - 2;
-    float4 next[kEach];
-    auto fetch = [&](int i) {
-      const int64_t k = static_cast<int64_t>(kb0 + i) * kBlockK + 4 * lane;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int t = w + 4 * e;
-        next[e] = t < p.tokens && k < p.ld_h ? __ldcg(reinterpret_cast<const float4 *>(p.h + t * p.ld_h + k)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      }
+      for (int a = 0; a < kRowsM / S::kFeatures; ++a)
+        tma_load_3d(stage + a * S::kFeatures * kBlockK, &p.w_map, (kb0 + i) * kBlockK, f0, a, bar, stream_once);
     };
-    fetch(0);
-    uint32_t top[kEach] = {};
-    for (int i = lane; i < p.h_tiles; i += 32)
-#pragma unroll
-      for (int e = 0; e < kEach; ++e)
-        if (w + 4 * e < p.tokens) top[e] = max(top[e], __ldcg(p.tile_max + static_cast<int64_t>(w + 4 * e) * p.h_tiles + i));
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const float s = int8_scale(__reduce_max_sync(0xffffffffu, top[e]));
-      if (lane == 0) {
-        row_scale[w + 4 * e] = s;
-        row_inverse[w + 4 * e] = s >= kTinyScale ? __fdiv_rn(1.0f, s) : 0.0f;
-      }
-    }
+    const int early = p.w_early ? min(n, S::kStages) : 0;
+    if (elect_one())
+      for (int i = 0; i < early; ++i) load_w(i);
     __syncwarp();
-    for (int i = 0; i < n; ++i) {
+    pdl_wait();
+    pdl_launch_dependents();
+    int i = 0;
+    for (; i < n; ++i) {
       const int s = i % S::kStages;
-      float4 v[kEach];
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) v[e] = next[e];
-      if (i + 1 < n) fetch(i + 1);
       if (i >= S::kStages &&
           !warp_agrees(mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty)))
         break;
-      uint8_t *codes = ring_ptr + s * S::kStageBytes + kBoxBytes;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        const int t = w + 4 * e;
-        if (t >= p.tokens) continue;
-        const float rs = row_scale[t], ri = row_inverse[t];
-        uint32_t word;
-        if (rs >= kTinyScale)
-          word = pack4(int8_code(v[e].x, rs, ri), int8_code(v[e].y, rs, ri), int8_code(v[e].z, rs, ri), int8_code(v[e].w, rs, ri));
-        else if (rs == rs)
-          word = pack4(int8_code_tiny(v[e].x, rs), int8_code_tiny(v[e].y, rs), int8_code_tiny(v[e].z, rs), int8_code_tiny(v[e].w, rs));
-        else
-          word = 0u;
-        // as TMA would place it: 16-byte units XORed with the row
-        *reinterpret_cast<uint32_t *>(codes + t * kBlockK + (((lane >> 2) ^ (t & 7)) << 4) + (lane & 3) * 4) = word;
+      if (elect_one()) {
+        if (i >= early) load_w(i);
+        tma_load_2d(ring + s * S::kStageBytes + kBoxBytes, &p.x_map, (kb0 + i) * kBlockK, 0, full + 8 * s, keep);
       }
-      fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(full + 8 * s);
     }
+    // leave no copy in flight, whatever ended the loop
+    for (int j = max(0, i - S::kStages); j < i; ++j) mbar_wait_drain(full + 8 * (j % S::kStages), (j / S::kStages) & 1);
+    __syncwarp();
+  } else if (warp == 1) {
+    constexpr uint32_t idesc = idesc_i8(kRowsM, BN);
+    for (int i = 0; i < n; ++i) {
+      const int s = i % S::kStages;
+      if (!warp_agrees(mbar_wait(full + 8 * s, (i / S::kStages) & 1, &g_int8_error, kErrTimeoutFull))) {
+        *failed = 1u;
+        break;
+      }
+      tc_fence_after();
+      const uint32_t stage = ring + s * S::kStageBytes;
+      const uint64_t w = smem_desc(stage, 16, 1024, kLayoutSw128);
+      const uint64_t b = smem_desc(stage + kBoxBytes, 16, 1024, kLayoutSw128);
+      if (elect_one()) {
+#pragma unroll
+        for (int k = 0; k < kBlockK / 32; ++k)  // 32 bytes of depth an instruction
+          tc_mma_i8(tmem, w + 2 * k, b + 2 * k, idesc, i > 0 || k > 0);
+        tc_commit(empty + 8 * s);
+      }
+      __syncwarp();
+    }
+    if (elect_one()) tc_commit(acc);
+    __syncwarp();
+    mbar_wait_drain(acc, 0);
     __syncwarp();
   }
 
   // Every warp takes part in the reduction; warps 2..5 first bring the sums from TMEM (warp w
   // reads lanes 32 (w % 4) and on: weight rows) into the ring's place, token-major.
-  if (KIND == kRequant && warp == 0) {
-    pdl_wait();
-    pdl_launch_dependents();
-  }
   // a lane finishes PER neighbouring features of a token
   constexpr int PER = S::kFeatures / 32;
   const int es = p.out_type == MM_DTYPE_FP32 ? 4 : 2;
@@ -358,7 +284,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       }
     }
     const int64_t t = j;
-    const float xs = KIND == kRequant ? row_scale[t] : p.x_scale[t];
+    const float xs = p.x_scale[t];
     const float a[4] = {__fmul_rn(static_cast<float>(sum.x), xs), __fmul_rn(static_cast<float>(sum.y), xs),
                         __fmul_rn(static_cast<float>(sum.z), xs), __fmul_rn(static_cast<float>(sum.w), xs)};
     float v[PER];
@@ -368,14 +294,6 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       else v[i] = __fmaf_rn(a[i], ws[i], second[i]);
     }
     if (ok && left > 0) store_some<PER>(p, t * p.ld_out + f, left, v, wide);
-    if (GATED && p.tile_max != nullptr) {
-      uint32_t top = 0u;
-#pragma unroll
-      for (int i = 0; i < PER; ++i)
-        if (i < left) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-      top = __reduce_max_sync(0xffffffffu, top);
-      if (lane == 0) p.tile_max[static_cast<int64_t>(t) * p.h_tiles + f0 / S::kFeatures] = top;
-    }
   }
   // the parts are read: the CTA may end
   if (split > 1) cluster_sync();
@@ -458,43 +376,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
   pdl_launch_dependents();  // after the allocation, as in the stream form
 
   if (warp == 0) {
-    {
-      pdl_wait();
-      const uint32_t block_tx = 2 * (kBoxBytes + half_n * kBlockK);  // both CTAs' bytes
-      int it = 0;
-      bool ok = true;
-      for (int tile = pair; tile < tiles && ok; tile += pairs) {
-        int tt, ft;
-        tile_at(p, tile, tt, ft);
-        const int t0 = tt * kTileM + rank * kRowsM;
-        const int row = GATED ? ft * tile_f : ft * tile_f + rank * half_n, plane = GATED ? rank : 0;
-        for (int kb = 0; kb < p.blocks_k; kb += kTileBlocks, ++it) {
-          const int s = it % kTileStages;
-          if (it >= kTileStages &&
-              !warp_agrees(mbar_wait_cluster(empty + 8 * s, ((it / kTileStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty))) {
-            ok = false;
-            break;
-          }
-          const uint32_t stage = ring + s * kTileStageBytes;
-          // the leader's barrier counts the bytes of both CTAs: this CTA's copies may land
-          // there before the leader expects them, the phase still ends with its arrival
-          const uint32_t bar = cluster_map(full + 8 * s, 0);
-          const int blocks = min(kTileBlocks, p.blocks_k - kb);
-          if (elect_one()) {
-            if (rank == 0) mbar_expect_tx(full + 8 * s, blocks * block_tx);
-            for (int j = 0; j < blocks; ++j) {
-              tma_pair_load_2d(stage + 2 * j * kBoxBytes, &p.x_map, (kb + j) * kBlockK, t0, bar);
-              tma_pair_load_3d(stage + (2 * j + 1) * kBoxBytes, &p.w_map, (kb + j) * kBlockK, row, plane, bar);
-            }
-          }
-          __syncwarp();
+    pdl_wait();
+    const uint32_t block_tx = 2 * (kBoxBytes + half_n * kBlockK);  // both CTAs' bytes
+    int it = 0;
+    bool ok = true;
+    for (int tile = pair; tile < tiles && ok; tile += pairs) {
+      int tt, ft;
+      tile_at(p, tile, tt, ft);
+      const int t0 = tt * kTileM + rank * kRowsM;
+      const int row = GATED ? ft * tile_f : ft * tile_f + rank * half_n, plane = GATED ? rank : 0;
+      for (int kb = 0; kb < p.blocks_k; kb += kTileBlocks, ++it) {
+        const int s = it % kTileStages;
+        if (it >= kTileStages &&
+            !warp_agrees(mbar_wait_cluster(empty + 8 * s, ((it / kTileStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty))) {
+          ok = false;
+          break;
         }
+        const uint32_t stage = ring + s * kTileStageBytes;
+        // the leader's barrier counts the bytes of both CTAs: this CTA's copies may land
+        // there before the leader expects them, the phase still ends with its arrival
+        const uint32_t bar = cluster_map(full + 8 * s, 0);
+        const int blocks = min(kTileBlocks, p.blocks_k - kb);
+        if (elect_one()) {
+          if (rank == 0) mbar_expect_tx(full + 8 * s, blocks * block_tx);
+          for (int j = 0; j < blocks; ++j) {
+            tma_pair_load_2d(stage + 2 * j * kBoxBytes, &p.x_map, (kb + j) * kBlockK, t0, bar);
+            tma_pair_load_3d(stage + (2 * j + 1) * kBoxBytes, &p.w_map, (kb + j) * kBlockK, row, plane, bar);
+          }
+        }
+        __syncwarp();
       }
-      // leave no copy in flight: the last stages' barriers complete with both CTAs' copies
-      if (rank == 0)
-        for (int j = max(0, it - kTileStages); j < it; ++j)
-          mbar_wait_drain(full + 8 * (j % kTileStages), (j / kTileStages) & 1);
     }
+    // leave no copy in flight: the last stages' barriers complete with both CTAs' copies
+    if (rank == 0)
+      for (int j = max(0, it - kTileStages); j < it; ++j)
+        mbar_wait_drain(full + 8 * (j % kTileStages), (j / kTileStages) & 1);
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0) {
@@ -700,18 +616,18 @@ cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, int clust
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-template <int BN, int KIND>
+template <int BN, bool GATED>
 cudaError_t launch_stream(Int8Args &a, void *stream) {
-  using S = Stream<BN, KIND>;
+  using S = Stream<BN, GATED>;
   static bool done[64] = {};
-  const cudaError_t e = raise_smem(int8_stream_kernel<BN, KIND>, S::kSmem, done);
+  const cudaError_t e = raise_smem(int8_stream_kernel<BN, GATED>, S::kSmem, done);
   if (e != cudaSuccess) return e;
   const int tiles = (a.features + S::kFeatures - 1) / S::kFeatures;
   // enough CTAs for two an SM, each with at least two stages of depth
   int split = 1;
   while (split < 8 && tiles * split < 148 && 4 * split <= a.blocks_k) split *= 2;
   a.split = split;
-  return launch_cluster(int8_stream_kernel<BN, KIND>, dim3(tiles * split), kStreamThreads, S::kSmem, split, stream, a);
+  return launch_cluster(int8_stream_kernel<BN, GATED>, dim3(tiles * split), kStreamThreads, S::kSmem, split, stream, a);
 }
 
 // CTA pairs that the current device runs at once (of the tile form: one CTA an SM, all its
@@ -768,8 +684,7 @@ struct Product {
   bool gated;
   float clamp;
   bool out_pad;         // the columns from features to ld_out may be written
-  uint32_t *tile_max;   // gated: [tokens, tiles] maxima out; else with h: the requantizing form
-  const float *h;       // in place of x and x_scale, rows ld_x values apart
+  bool w_early;         // see Int8Args
 };
 
 int check(const char *what, const Product &q) {
@@ -781,7 +696,7 @@ int check(const char *what, const Product &q) {
   if (q.out_type != MM_DTYPE_BF16 && q.out_type != MM_DTYPE_FP16 && q.out_type != MM_DTYPE_FP32)
     return set_error(MM_ERR_INVALID, "%s: unknown output type %d", what, q.out_type);
   if (q.tokens == 0) return MM_OK;
-  if (!(q.h || (q.x && q.x_scale)) || !q.w || !q.w_scale || !q.out) return set_error(MM_ERR_INVALID, "%s: null pointer", what);
+  if (!q.x || !q.x_scale || !q.w || !q.w_scale || !q.out) return set_error(MM_ERR_INVALID, "%s: null pointer", what);
   if (q.ld_x < q.depth || q.ld_w < q.depth || q.ld_out < q.features)
     return set_error(MM_ERR_INVALID, "%s: a row stride below the row's length", what);
   if (!aligned(q.x, 16) || !aligned(q.w, 16) || q.ld_x % 16 || q.ld_w % 16)
@@ -805,10 +720,7 @@ int run(const char *what, const Product &q, void *stream) {
   a.gated = q.gated;
   a.has_clamp = q.clamp > 0.0f;
   a.clamp = q.clamp;
-  a.h = q.h;
-  a.ld_h = q.ld_x;
-  a.tile_max = q.tile_max;
-  a.h_tiles = ((q.gated ? q.features : q.depth) + kRowsM / 2 - 1) / (kRowsM / 2);
+  a.w_early = q.w_early;
   auto w_map = [&](int rows) { return encode(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, q.depth, q.features, q.gated ? 2 : 1, q.ld_w, rows); };
   int rc;
   auto x_map = [&](int rows) { return encode(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, q.depth, q.tokens, 0, q.ld_x, rows); };
@@ -845,22 +757,18 @@ int run(const char *what, const Product &q, void *stream) {
     return MM_OK;
   }
   if ((rc = w_map(q.gated ? kRowsM / 2 : kRowsM))) return rc;
-  if (q.h) {
-    if ((e = launch_stream<16, kRequant>(a, stream)) != cudaSuccess) return set_error(MM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
-    return MM_OK;
-  }
   int bn = 16;
   while (bn < q.tokens) bn *= 2;
   if ((rc = x_map(bn))) return rc;
   switch (q.gated ? -bn : bn) {
-    case 16: e = launch_stream<16, kLinear>(a, stream); break;
-    case 32: e = launch_stream<32, kLinear>(a, stream); break;
-    case 64: e = launch_stream<64, kLinear>(a, stream); break;
-    case 128: e = launch_stream<128, kLinear>(a, stream); break;
-    case -16: e = launch_stream<16, kGated>(a, stream); break;
-    case -32: e = launch_stream<32, kGated>(a, stream); break;
-    case -64: e = launch_stream<64, kGated>(a, stream); break;
-    default: e = launch_stream<128, kGated>(a, stream); break;
+    case 16: e = launch_stream<16, false>(a, stream); break;
+    case 32: e = launch_stream<32, false>(a, stream); break;
+    case 64: e = launch_stream<64, false>(a, stream); break;
+    case 128: e = launch_stream<128, false>(a, stream); break;
+    case -16: e = launch_stream<16, true>(a, stream); break;
+    case -32: e = launch_stream<32, true>(a, stream); break;
+    case -64: e = launch_stream<64, true>(a, stream); break;
+    default: e = launch_stream<128, true>(a, stream); break;
   }
   if (e != cudaSuccess) return set_error(MM_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
   return MM_OK;
@@ -878,7 +786,7 @@ extern "C" {
 int mm_int8_linear(const int8_t *x, int64_t ld_x, const float *x_scale, const int8_t *w, int64_t ld_w,
                    const float *w_scale, const float *bias, void *out, int64_t ld_out, int32_t out_dtype,
                    int32_t tokens, int32_t features, int32_t depth, void *stream) {
-  const Product q = {x, ld_x, x_scale, w, ld_w, w_scale, bias, out, ld_out, out_dtype, tokens, features, depth, false, 0.0f, false, nullptr, nullptr};
+  const Product q = {x, ld_x, x_scale, w, ld_w, w_scale, bias, out, ld_out, out_dtype, tokens, features, depth, false, 0.0f, false, false};
   const int rc = check("mm_int8_linear", q);
   if (rc || tokens == 0) return rc;
   return run("mm_int8_linear", q, stream);
@@ -898,29 +806,21 @@ int mm_int8_ffn(const mm_int8_ffn_args *f, void *stream) {
   if (f->tokens > 0 && (!ws || !aligned(ws, 256) || f->workspace_bytes < mm_int8_ffn_workspace(f->tokens, f->inter)))
     return set_error(MM_ERR_INVALID, "mm_int8_ffn: the workspace needs %lld bytes on a 256-byte boundary",
                      static_cast<long long>(mm_int8_ffn_workspace(f->tokens, f->inter)));
-  // h in fp32 (its rounding to int8 is the only one), rows on 16-byte boundaries; then its codes
-  // and scales, or few tokens' tile maxima in their place
+  // h in fp32 (its rounding to int8 is the only one), rows on 16-byte boundaries; its codes; scales
   const int64_t ld_h = up(f->inter, 4), ld_q = up(f->inter, 16);
   float *h = reinterpret_cast<float *>(ws);
   int8_t *hq = ws ? reinterpret_cast<int8_t *>(ws + up(f->tokens * ld_h * 4, 256)) : nullptr;
   float *hs = ws ? reinterpret_cast<float *>(hq + up(f->tokens * ld_q, 256)) : nullptr;
-  const bool few = f->tokens <= kRequantTokens;
   const Product up_q = {f->x, f->ld_x, f->x_scale, f->w13, f->ld_w13, f->w13_scale, nullptr, h, ld_h, MM_DTYPE_FP32,
-                        f->tokens, f->inter, f->hidden, true, f->clamp, true,
-                        few ? reinterpret_cast<uint32_t *>(hq) : nullptr, nullptr};
-  Product down_q = {hq, ld_q, hs, f->w2, f->ld_w2, f->w2_scale, nullptr, f->out, f->ld_out, f->out_dtype,
-                    f->tokens, f->hidden, f->inter, false, 0.0f, false, nullptr, nullptr};
+                        f->tokens, f->inter, f->hidden, true, f->clamp, true, false};
+  // the down product's predecessors, the row kernel and the gated product, do not write w2
+  const Product down_q = {hq, ld_q, hs, f->w2, f->ld_w2, f->w2_scale, nullptr, f->out, f->ld_out, f->out_dtype,
+                          f->tokens, f->hidden, f->inter, false, 0.0f, false, true};
   int rc = check("mm_int8_ffn", up_q);
   if (!rc) rc = check("mm_int8_ffn", down_q);
   if (rc || f->tokens == 0) return rc;
   if ((rc = run("mm_int8_ffn", up_q, stream))) return rc;
-  if (few) {
-    down_q.h = h;
-    down_q.ld_x = ld_h;
-    down_q.tile_max = up_q.tile_max;
-  } else if ((rc = quantize_rows("mm_int8_ffn", h, ld_h, MM_DTYPE_FP32, hq, ld_q, hs, f->tokens, f->inter, stream))) {
-    return rc;
-  }
+  if ((rc = quantize_rows("mm_int8_ffn", h, ld_h, MM_DTYPE_FP32, hq, ld_q, hs, f->tokens, f->inter, stream))) return rc;
   return run("mm_int8_ffn", down_q, stream);
 }
 
