@@ -11,8 +11,8 @@
 //  * int8_stream_kernel (few tokens; bound by the weights' stream). 128 weight rows are the
 //    MMA's M side and up to 128 tokens its N side, so one token costs one column and the
 //    tokens' padding costs no memory traffic. Few tiles do not fill the GPU: the CTAs of a
-//    cluster share a tile's depth, and add their integer parts through distributed shared
-//    memory, each finishing its share of the tokens. No workspace, no atomics, no counters.
+//    cluster share a tile's depth, and send their integer parts through distributed shared
+//    memory, each adding and finishing its share of the tokens. No workspace, no atomics, no counters.
 //  * int8_tile_kernel (many tokens; bound by the tensor pipe). A CTA pair owns 256 tokens x
 //    256 weight rows (cta_group::2: each CTA stages half of either operand, half the shared
 //    memory traffic of two single tiles), persistent, with two accumulators in TMEM so that
@@ -61,7 +61,7 @@ struct alignas(64) Int8Args {
   float clamp;
   int token_tiles, feature_tiles, tile_n;  // of the tile form
   int w_early;          // the launch's predecessors do not write the weights: load before waiting
-  int split;            // CTAs of a cluster that share a tile's depth (stream form)
+  int split;            // CTAs of a cluster that share a tile's depth (stream form), a power of two
 };
 
 // A whole warp waits, one elected lane issues: the lanes go on together, or give up together.
@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   const uint32_t ring = (raw + 1023u) & ~1023u;
   uint8_t *ring_ptr = smem_raw + (ring - raw);
   const uint32_t bars = ring + S::kStages * S::kStageBytes;
-  const uint32_t full = bars, empty = bars + 8 * S::kStages, acc = bars + 16 * S::kStages, slot = acc + 8;
+  const uint32_t full = bars, empty = bars + 8 * S::kStages, acc = bars + 16 * S::kStages, recv = acc + 8, slot = recv + 8;
+  __shared__ float x_scale[BN];
   uint32_t *slot_ptr = reinterpret_cast<uint32_t *>(ring_ptr + (slot - ring));
   volatile uint32_t *failed = slot_ptr + 1;
 
@@ -159,8 +160,12 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       mbar_init(empty + 8 * s, 1);
     }
     mbar_init(acc, 1);
+    mbar_init(recv, 1);
     *failed = 0u;
     fence_barrier_init();
+    // this CTA finishes the tokens rank, rank + split, ...: a part of each from every CTA
+    const int mine = (p.tokens - rank + split - 1) / split;
+    if (split > 1 && mine > 0) mbar_expect_tx(recv, mine * split * kRowsM * 4);
   }
   if (warp == 1) {
     tmem_alloc(slot, S::kCols);
@@ -236,8 +241,6 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     __syncwarp();
   }
 
-  // Every warp takes part in the reduction; warps 2..5 first bring the sums from TMEM (warp w
-  // reads lanes 32 (w % 4) and on: weight rows) into the ring's place, token-major.
   // a lane finishes PER neighbouring features of a token
   constexpr int PER = S::kFeatures / 32;
   const int es = p.out_type == MM_DTYPE_FP32 ? 4 : 2;
@@ -250,41 +253,64 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     ws[i] = i < left ? p.w_scale[f + i] : 0.0f;
     second[i] = i >= left ? 0.0f : GATED ? p.w_scale[static_cast<int64_t>(p.features) + f + i] : p.bias ? p.bias[f + i] : 0.0f;
   }
+  if (warp >= 2 && threadIdx.x - 64 < p.tokens) x_scale[threadIdx.x - 64] = p.x_scale[threadIdx.x - 64];
   bool ok = mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc);
   tc_fence_after();
   ok = ok && *failed == 0u;
+  // The parts go to the CTA that finishes their token, into its ring once every CTA of the
+  // cluster is past its products: [token's turn][part][weight row]. Warps 2..5 send; warp w
+  // reads TMEM lanes 32 (w % 4) and on, weight rows, a column a token.
+  const int turns = __ffs(split) - 1;  // split is a power of two
+  if (split > 1) cluster_arrive();
   if (warp >= 2) {
     const int q = warp & 3;
+    const uint32_t at = ring + (rank * kRowsM + q * 32 + lane) * 4;
 #pragma unroll 1
     for (int j = 0; j < p.tokens; j += 16) {
       uint32_t r[16];
       tc_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + j, r);
       tc_wait_ld();
-      uint32_t *to = reinterpret_cast<uint32_t *>(ring_ptr) + j * kRowsM + q * 32 + lane;
+      if (split > 1) {
+        if (j == 0) cluster_wait();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) to[i * kRowsM] = r[i];
+        for (int i = 0; i < 16; ++i) {
+          const int owner = (j + i) & (split - 1), turn = (j + i) >> turns;
+          if (j + i < p.tokens)
+            cluster_store_async(cluster_map(at + turn * split * kRowsM * 4, owner), r[i], cluster_map(recv, owner));
+        }
+      } else {
+        uint32_t *to = reinterpret_cast<uint32_t *>(ring_ptr + (at - ring)) + j * kRowsM;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) to[i * kRowsM] = r[i];
+      }
     }
+  } else if (split > 1) {
+    cluster_wait();
   }
-  if (split > 1) cluster_sync();
-  else __syncthreads();
+  tc_fence_before();
+  __syncthreads();  // x's scales, one CTA's parts, and the TMEM reads
+  if (warp == 1) tmem_dealloc(tmem, S::kCols);
+  if (split > 1 && rank < p.tokens && !mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc)) {
+    cluster_sync();  // parts may still come: stay until their senders are gone
+    return;
+  }
 #pragma unroll 1
-  for (int j = rank * kStreamWarps + warp; j < p.tokens; j += split * kStreamWarps) {
+  for (int j = rank + split * warp; j < p.tokens; j += split * kStreamWarps) {
     // the parts of four sums: four features, or two features' gate and up
-    const uint32_t at = ring + (j * kRowsM + PER * lane) * 4;
+    const int *part = reinterpret_cast<const int *>(ring_ptr) + (j & ~(split - 1)) * kRowsM + PER * lane;
     int4 sum = make_int4(0, 0, 0, 0);
-#pragma unroll 4
-    for (int r = 0; r < split; ++r) {
-      const uint32_t from = cluster_map(at, r);
+#pragma unroll 8
+    for (int r = 0; r < split; ++r, part += kRowsM) {
       if constexpr (GATED) {
-        const int2 g = cluster_load_v2(from), u = cluster_load_v2(from + 4 * S::kFeatures);
+        const int2 g = *reinterpret_cast<const int2 *>(part), u = *reinterpret_cast<const int2 *>(part + S::kFeatures);
         sum.x += g.x, sum.y += g.y, sum.z += u.x, sum.w += u.y;
       } else {
-        const int4 v = cluster_load_v4(from);
+        const int4 v = *reinterpret_cast<const int4 *>(part);
         sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
       }
     }
     const int64_t t = j;
-    const float xs = p.x_scale[t];
+    const float xs = x_scale[j];
     const float a[4] = {__fmul_rn(static_cast<float>(sum.x), xs), __fmul_rn(static_cast<float>(sum.y), xs),
                         __fmul_rn(static_cast<float>(sum.z), xs), __fmul_rn(static_cast<float>(sum.w), xs)};
     float v[PER];
@@ -295,12 +321,6 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     }
     if (ok && left > 0) store_some<PER>(p, t * p.ld_out + f, left, v, wide);
   }
-  // the parts are read: the CTA may end
-  if (split > 1) cluster_sync();
-  else __syncthreads();
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) tmem_dealloc(tmem, S::kCols);
 }
 
 // ---------------------------------------------------------------------------------------
