@@ -11,7 +11,7 @@
 //  * int8_stream_kernel (few tokens; bound by the weights' stream). 128 weight rows are the
 //    MMA's M side and up to 128 tokens its N side, so one token costs one column and the
 //    tokens' padding costs no memory traffic. Few tiles do not fill the GPU: the CTAs of a
-//    cluster share a tile's depth, and send their integer parts through distributed shared
+//    cluster share a tile's depth and exchange their integer parts through distributed shared
 //    memory, each adding and finishing its share of the tokens. No workspace, no atomics, no counters.
 //  * int8_tile_kernel (many tokens; bound by the tensor pipe). A CTA pair owns 256 tokens x
 //    256 weight rows (cta_group::2: each CTA stages half of either operand, half the shared
@@ -120,6 +120,10 @@ struct Stream {
   static constexpr int kStages = kRing / kStageBytes;
   static constexpr int kCols = BN < 32 ? 32 : BN;  // TMEM columns, a power of two
   static constexpr int kSmem = kStages * kStageBytes + 1024 + 256;
+  // Parts are sent where they are few and read where they are many (us, sent against read: 1 x
+  // 4096 x 7168 7.3 and 7.7, 16 x 7168 x 7168 10.6 and 11.0, 64 x 7168 x 7168 12.9 and 12.4, 128 x
+  // 7168 x 7168 16.5 and 15.0): a send moves 4 bytes a lane, a read 16.
+  static constexpr bool kPush = BN <= 32;
   static_assert(kStages >= 2 && kCols <= 256, "two CTAs an SM share 512 columns");
   static_assert(BN * kRowsM * 4 <= kStages * kStageBytes, "the parts take the ring's place");
 };
@@ -163,9 +167,9 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     mbar_init(recv, 1);
     *failed = 0u;
     fence_barrier_init();
-    // this CTA finishes the tokens rank, rank + split, ...: a part of each from every CTA
+    // a part of each token that this CTA finishes, from every CTA
     const int mine = (p.tokens - rank + split - 1) / split;
-    if (split > 1 && mine > 0) mbar_expect_tx(recv, mine * split * kRowsM * 4);
+    if (S::kPush && split > 1 && mine > 0) mbar_expect_tx(recv, mine * split * kRowsM * 4);
   }
   if (warp == 1) {
     tmem_alloc(slot, S::kCols);
@@ -257,59 +261,11 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   bool ok = mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc);
   tc_fence_after();
   ok = ok && *failed == 0u;
-  // The parts go to the CTA that finishes their token, into its ring once every CTA of the
-  // cluster is past its products: [token's turn][part][weight row]. Warps 2..5 send; warp w
-  // reads TMEM lanes 32 (w % 4) and on, weight rows, a column a token.
-  const int turns = __ffs(split) - 1;  // split is a power of two
-  if (split > 1) cluster_arrive();
-  if (warp >= 2) {
-    const int q = warp & 3;
-    const uint32_t at = ring + (rank * kRowsM + q * 32 + lane) * 4;
-#pragma unroll 1
-    for (int j = 0; j < p.tokens; j += 16) {
-      uint32_t r[16];
-      tc_ld_32x32b_x16(tmem + (static_cast<uint32_t>(q * 32) << 16) + j, r);
-      tc_wait_ld();
-      if (split > 1) {
-        if (j == 0) cluster_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int owner = (j + i) & (split - 1), turn = (j + i) >> turns;
-          if (j + i < p.tokens)
-            cluster_store_async(cluster_map(at + turn * split * kRowsM * 4, owner), r[i], cluster_map(recv, owner));
-        }
-      } else {
-        uint32_t *to = reinterpret_cast<uint32_t *>(ring_ptr + (at - ring)) + j * kRowsM;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) to[i * kRowsM] = r[i];
-      }
-    }
-  } else if (split > 1) {
-    cluster_wait();
-  }
-  tc_fence_before();
-  __syncthreads();  // x's scales, one CTA's parts, and the TMEM reads
-  if (warp == 1) tmem_dealloc(tmem, S::kCols);
-  if (split > 1 && rank < p.tokens && !mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc)) {
-    cluster_sync();  // parts may still come: stay until their senders are gone
-    return;
-  }
-#pragma unroll 1
-  for (int j = rank + split * warp; j < p.tokens; j += split * kStreamWarps) {
-    // the parts of four sums: four features, or two features' gate and up
-    const int *part = reinterpret_cast<const int *>(ring_ptr) + (j & ~(split - 1)) * kRowsM + PER * lane;
-    int4 sum = make_int4(0, 0, 0, 0);
-#pragma unroll 8
-    for (int r = 0; r < split; ++r, part += kRowsM) {
-      if constexpr (GATED) {
-        const int2 g = *reinterpret_cast<const int2 *>(part), u = *reinterpret_cast<const int2 *>(part + S::kFeatures);
-        sum.x += g.x, sum.y += g.y, sum.z += u.x, sum.w += u.y;
-      } else {
-        const int4 v = *reinterpret_cast<const int4 *>(part);
-        sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-      }
-    }
-    const int64_t t = j;
+  // Every CTA of the cluster finishes the tokens rank, rank + split, ... Warps 2..5 read the sums
+  // (warp w: TMEM lanes 32 (w % 4) and on, weight rows; a column a token).
+  const int q = warp & 3;
+  const uint32_t sums = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  auto finish = [&](int j, int4 sum) {
     const float xs = x_scale[j];
     const float a[4] = {__fmul_rn(static_cast<float>(sum.x), xs), __fmul_rn(static_cast<float>(sum.y), xs),
                         __fmul_rn(static_cast<float>(sum.z), xs), __fmul_rn(static_cast<float>(sum.w), xs)};
@@ -319,8 +275,89 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       if constexpr (GATED) v[i] = gate_up(p, __fmul_rn(a[i], ws[i]), __fmul_rn(a[PER + i], second[i]));
       else v[i] = __fmaf_rn(a[i], ws[i], second[i]);
     }
-    if (ok && left > 0) store_some<PER>(p, t * p.ld_out + f, left, v, wide);
+    if (ok && left > 0) store_some<PER>(p, j * p.ld_out + f, left, v, wide);
+  };
+  // the four sums of a lane: four features, or two features' gate and up
+  auto add = [](int4 &sum, const int4 &v) { sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w; };
+  if (S::kPush && split > 1) {
+    // The parts go into the ring of the CTA that finishes their token, once every CTA of the
+    // cluster is past its products: [token's turn][part][weight row].
+    cluster_arrive();
+    if (warp >= 2) {
+      const int turns = __ffs(split) - 1;  // split is a power of two
+      const uint32_t at = ring + (rank * kRowsM + q * 32 + lane) * 4;
+#pragma unroll 1
+      for (int j = 0; j < p.tokens; j += 16) {
+        uint32_t r[16];
+        tc_ld_32x32b_x16(sums + j, r);
+        tc_wait_ld();
+        if (j == 0) cluster_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int owner = (j + i) & (split - 1), turn = (j + i) >> turns;
+          if (j + i < p.tokens)
+            cluster_store_async(cluster_map(at + turn * split * kRowsM * 4, owner), r[i], cluster_map(recv, owner));
+        }
+      }
+    } else {
+      cluster_wait();
+    }
+    tc_fence_before();
+    __syncthreads();  // x's scales, and the TMEM reads
+    if (warp == 1) tmem_dealloc(tmem, S::kCols);
+    if (rank < p.tokens && !mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc)) {
+      cluster_sync();  // parts may still come: stay until their senders are gone
+      return;
+    }
+#pragma unroll 1
+    for (int j = rank + split * warp; j < p.tokens; j += split * kStreamWarps) {
+      const int *part = reinterpret_cast<const int *>(ring_ptr) + (j & ~(split - 1)) * kRowsM + PER * lane;
+      int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 8
+      for (int r = 0; r < split; ++r, part += kRowsM) {
+        if constexpr (GATED) {
+          const int2 g = *reinterpret_cast<const int2 *>(part), u = *reinterpret_cast<const int2 *>(part + S::kFeatures);
+          add(sum, make_int4(g.x, g.y, u.x, u.y));
+        } else {
+          add(sum, *reinterpret_cast<const int4 *>(part));
+        }
+      }
+      finish(j, sum);
+    }
+    return;
   }
+  // Each CTA leaves its parts in its own ring, [token][weight row], and reads the others' there.
+  if (warp >= 2) {
+#pragma unroll 1
+    for (int j = 0; j < p.tokens; j += 16) {
+      uint32_t r[16];
+      tc_ld_32x32b_x16(sums + j, r);
+      tc_wait_ld();
+      uint32_t *to = reinterpret_cast<uint32_t *>(ring_ptr) + j * kRowsM + q * 32 + lane;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) to[i * kRowsM] = r[i];
+    }
+  }
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 1) tmem_dealloc(tmem, S::kCols);
+#pragma unroll 1
+  for (int j = rank + split * warp; j < p.tokens; j += split * kStreamWarps) {
+    const uint32_t at = ring + (j * kRowsM + PER * lane) * 4;
+    int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int r = 0; r < split; ++r) {
+      const uint32_t from = cluster_map(at, r);
+      if constexpr (GATED) {
+        const int2 g = cluster_load_v2(from), u = cluster_load_v2(from + 4 * S::kFeatures);
+        add(sum, make_int4(g.x, g.y, u.x, u.y));
+      } else {
+        add(sum, cluster_load_v4(from));
+      }
+    }
+    finish(j, sum);
+  }
+  cluster_sync();  // the parts are read: the CTA may end
 }
 
 // ---------------------------------------------------------------------------------------

@@ -305,6 +305,17 @@ __device__ __forceinline__ uint32_t cluster_map(uint32_t addr, uint32_t rank) {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// Load from another CTA's shared memory (mapped address); ordered by the cluster barriers.
+__device__ __forceinline__ int4 cluster_load_v4(uint32_t mapped_addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(mapped_addr));
+  return v;
+}
+__device__ __forceinline__ int2 cluster_load_v2(uint32_t mapped_addr) {
+  int2 v;
+  asm volatile("ld.shared::cluster.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(mapped_addr));
+  return v;
+}
 // Store to another CTA's shared memory, its bytes counted on a barrier there (both mapped).
 __device__ __forceinline__ void cluster_store_async(uint32_t mapped_addr, uint32_t value, uint32_t mapped_bar) {
   asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(mapped_addr),
