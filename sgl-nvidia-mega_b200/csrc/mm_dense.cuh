@@ -19,6 +19,7 @@ struct NormArgs {
   uint8_t *codes;            // [tokens, ld_codes] 8-bit codes, or null
   void *scales;              // E8M0 [tokens, hidden / 32] or fp32 [tokens]
   int64_t ld_x, ld_residual, ld_residual_out, ld_norm, ld_codes;
+  double inv_n;              // 1 / hidden
   int tokens, hidden;
   float eps;
   int gamma_f32;             // gamma is fp32 beside a 16-bit x

@@ -97,29 +97,30 @@ __device__ __forceinline__ void store_codes(uint8_t *row, int e0, int n, const u
   }
 }
 
-// gamma's values of one chunk: its rows start wherever its own alignment says.
+// fp32 gamma beside a 16-bit x.
+template <int VEC>
+__device__ __forceinline__ void load_gamma_f32(const NormArgs &a, int e0, float (&g)[VEC]) {
+  const float *p = static_cast<const float *>(a.gamma);
+  if (VEC > 1 && a.gamma_wide && e0 % 4 == 0 && e0 >= 0 && e0 + VEC <= a.hidden) {
+#pragma unroll
+    for (int i = 0; i < VEC / 4; ++i) {
+      const float4 q = *reinterpret_cast<const float4 *>(p + e0 + 4 * i);
+      g[4 * i] = q.x, g[4 * i + 1] = q.y, g[4 * i + 2] = q.z, g[4 * i + 3] = q.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) g[i] = e0 + i >= 0 && e0 + i < a.hidden ? p[e0 + i] : 0.0f;
+}
+// gamma's values of one chunk, element by element.
 template <typename T, int VEC>
 __device__ __forceinline__ void load_gamma(const NormArgs &a, int e0, float (&g)[VEC]) {
   if (a.gamma_f32) {
-    const float *p = static_cast<const float *>(a.gamma);
-    if (VEC > 1 && a.gamma_wide && e0 % 4 == 0 && e0 >= 0 && e0 + VEC <= a.hidden) {
-#pragma unroll
-      for (int i = 0; i < VEC / 4; ++i) {
-        const float4 q = *reinterpret_cast<const float4 *>(p + e0 + 4 * i);
-        g[4 * i] = q.x, g[4 * i + 1] = q.y, g[4 * i + 2] = q.z, g[4 * i + 3] = q.w;
-      }
-      return;
-    }
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) g[i] = e0 + i >= 0 && e0 + i < a.hidden ? p[e0 + i] : 0.0f;
+    load_gamma_f32<VEC>(a, e0, g);
   } else {
     const T *p = static_cast<const T *>(a.gamma);
-    if (VEC > 1 && a.gamma_wide && (e0 * static_cast<int>(sizeof(T))) % 16 == 0) {
-      load_chunk<T, VEC>(p, e0, a.hidden, g);
-    } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) g[i] = e0 + i >= 0 && e0 + i < a.hidden ? Elem<T>::load(p + e0 + i) : 0.0f;
-    }
+    for (int i = 0; i < VEC; ++i) g[i] = e0 + i >= 0 && e0 + i < a.hidden ? Elem<T>::load(p + e0 + i) : 0.0f;
   }
 }
 
@@ -254,10 +255,10 @@ __device__ __forceinline__ uint32_t mx_code(uint32_t amax_bits) {
   return amax_bits == 0u ? 127u : min(c, 255u);
 }
 
-// 1 / sqrt(sum / n + eps): the sum's last steps and Newton's step in 64 bits, so that one
+// 1 / sqrt(sum * inv_n + eps): the sum's last steps and Newton's step in 64 bits, so that one
 // rounding is left in the factor that a whole row shares.
-__device__ __forceinline__ float inverse_rms(double sum, int n, float eps) {
-  const double m = sum / n + static_cast<double>(eps);
+__device__ __forceinline__ float inverse_rms(double sum, double inv_n, float eps) {
+  const double m = sum * inv_n + static_cast<double>(eps);
   const float y0 = rsqrtf(static_cast<float>(m));
   if (!(y0 > 0.0f && y0 < __uint_as_float(0x7f800000u))) return y0;  // 0, inf, NaN
   const double y = y0;
@@ -283,11 +284,43 @@ __device__ __forceinline__ double block_sum(double v, uint32_t &top, double *red
   return v;
 }
 
+// gamma's elements [e0, e0 + VEC) as they are stored (of x's type), zero outside the row. Rows
+// that start inside a 16-byte unit put their chunks across gamma's units: two loads, and the
+// wanted words shifted out of them.
+template <typename T>
+__device__ __forceinline__ uint4 gamma_chunk(const NormArgs &a, int e0) {
+  using C = Chunk<T>;
+  constexpr int VEC = C::kVec;
+  const T *p = static_cast<const T *>(a.gamma);
+  const int off = e0 & (VEC - 1), low = e0 - off;  // e0 may be negative: VEC is a power of two
+  if (a.gamma_wide && low >= 0 && (off ? low + 2 * VEC : low + VEC) <= a.hidden) {
+    const uint4 u = *reinterpret_cast<const uint4 *>(p + low);
+    if (off == 0) return u;
+    const uint4 v = *reinterpret_cast<const uint4 *>(p + low + VEC);
+    const int bits = off * static_cast<int>(sizeof(T)) * 8;
+    uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+    if (bits & 64) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (bits & 32) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    return make_uint4(__funnelshift_r(w[0], w[1], bits & 16), __funnelshift_r(w[1], w[2], bits & 16),
+                      __funnelshift_r(w[2], w[3], bits & 16), __funnelshift_r(w[3], w[4], bits & 16));
+  }
+  return e0 < a.hidden ? C::load(p, e0, a.hidden, false) : make_uint4(0u, 0u, 0u, 0u);
+}
+
 // One CTA per row, NV chunks of it a thread, held in registers. Four and more take more than
 // the 64 registers that 1024 threads leave each.
+// CTAs that shall share an SM: two of fp32 rows (h of a wide layer, 4096 x 18432: 70 us instead
+// of 92; 16-bit rows lose by it, 8192 x 7168 36 instead of 30), one of the latency form.
+constexpr int row_ctas(int nv, bool norm, int es) { return nv == 8 && !norm && es == 4 ? 2 : nv == 1 ? 1 : 0; }
 constexpr int row_threads(int nv, bool norm) { return nv >= 8 && norm ? 512 : nv >= 4 ? 640 : 1024; }
 template <typename T, int NV, int QUANT, bool NORM>
-__global__ void __launch_bounds__(row_threads(NV, NORM)) norm_rows_kernel(const __grid_constant__ NormArgs a) {
+__global__ void __launch_bounds__(row_threads(NV, NORM), row_ctas(NV, NORM, sizeof(T))) norm_rows_kernel(const __grid_constant__ NormArgs a) {
   using C = Chunk<T>;
   constexpr int VEC = C::kVec, PAIRS = C::kPairs;
   __shared__ double red_d[32];
@@ -328,15 +361,27 @@ __global__ void __launch_bounds__(row_threads(NV, NORM)) norm_rows_kernel(const 
     }
   }
 
-  // gamma's values of chunk j; zero outside the row
+  // gamma's values of chunk j; zero outside the row. One chunk a thread: loaded before the
+  // reduction, whose wait then covers them (with two, 1024 x 5120 took 9.7 us instead of 8.4).
+  constexpr bool EARLY = NORM && NV == 1;
+  uint4 held = make_uint4(0u, 0u, 0u, 0u);
+  if constexpr (EARLY)
+    if (!a.gamma_f32) held = gamma_chunk<T>(a, first);
   auto gammas = [&](int j, float (&g)[VEC]) {
     const int e0 = first + j * step;
-    if (e0 < n) {
-      load_gamma<T, VEC>(a, e0, g);
-    } else {
+    if (sizeof(T) == 2 && a.gamma_f32) {
+      if (e0 < n) {
+        load_gamma_f32<VEC>(a, e0, g);
+      } else {
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) g[i] = 0.0f;
+        for (int i = 0; i < VEC; ++i) g[i] = 0.0f;
+      }
+      return;
     }
+    F2 f[PAIRS];
+    C::values(EARLY ? held : gamma_chunk<T>(a, e0), f);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) g[i] = i & 1 ? f[i / 2].y : f[i / 2].x;
   };
 
   F2 inv = {1.0f, 1.0f};
@@ -362,7 +407,7 @@ __global__ void __launch_bounds__(row_threads(NV, NORM)) norm_rows_kernel(const 
       }
     }
     const double sum = block_sum(static_cast<double>(ss.x) + static_cast<double>(ss.y), top, red_d, red_u);
-    inv.x = inv.y = inverse_rms(sum, n, a.eps);
+    inv.x = inv.y = inverse_rms(sum, a.inv_n, a.eps);
   }
 
   // y of chunk j
@@ -523,7 +568,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
       sum += static_cast<double>(ss);
     }
     uint32_t none = 0u;
-    inv = inverse_rms(block_sum(sum, none, red_d, red_u), n, a.eps);
+    inv = inverse_rms(block_sum(sum, none, red_d, red_u), a.inv_n, a.eps);
   }
 
   // y of chunk c from its r
@@ -767,7 +812,7 @@ int mm_rms_norm(const mm_norm_args *n, void *stream) {
   a.x = n->x;
   a.residual = n->residual;
   a.gamma = n->gamma;
-  a.gamma_f32 = n->gamma_dtype == MM_DTYPE_FP32;
+  a.gamma_f32 = n->gamma_dtype == MM_DTYPE_FP32 && n->dtype != MM_DTYPE_FP32;
   a.residual_out = n->residual ? n->residual_out : nullptr;
   a.norm_out = n->norm_out;
   a.codes = static_cast<uint8_t *>(n->codes);
@@ -780,6 +825,7 @@ int mm_rms_norm(const mm_norm_args *n, void *stream) {
   a.tokens = n->tokens;
   a.hidden = n->hidden;
   a.eps = n->eps;
+  a.inv_n = n->hidden > 0 ? 1.0 / n->hidden : 0.0;
   return run_norm("mm_rms_norm", a, n->dtype, n->quant, stream);
 }
 
