@@ -351,6 +351,7 @@ class RoutedMoE:
         residual: Optional[torch.Tensor] = None,
         gamma: Optional[torch.Tensor] = None,
         alt=None,
+        shared_output: Optional[torch.Tensor] = None,
     ):
         """One whole MoE step on the current stream. Returns the bf16 [T, H]
         output (or the fp32 [2, T, H] partial sums with ``partial``; with
@@ -359,7 +360,9 @@ class RoutedMoE:
         ``comm`` and ``residual`` (bf16 [T, H]), the decoder hop's epilogue too:
         returns (norm_out, residual_out) as ``comm.moe_finalize_all_reduce_rms_norm``
         does, norm_out None without ``gamma``; residual_out may be ``residual``
-        itself via buffers["residual_out"]). ``buffers``
+        itself via buffers["residual_out"]). ``shared_output`` (bf16 [T, H], a
+        layer without a shared expert of its own): what the combine adds to the
+        routed sum, e.g. an ``int8_ffn`` of the same tokens. ``buffers``
         (optional dict) receives the intermediate tensors and may carry
         preallocated ones (keys: logits, weights, ids, permuted, record, rows,
         out, partial) so repeated calls allocate nothing."""
@@ -374,6 +377,12 @@ class RoutedMoE:
                 raise ValueError("residual must be contiguous bf16 [T, H]")
             if gamma is not None and (gamma.dtype != torch.bfloat16 or tuple(gamma.shape) != (self.hidden,)):
                 raise ValueError("gamma must be bf16 [H]")
+        if shared_output is not None:
+            if self.has_shared:
+                raise ValueError("forward: shared_output needs a layer without a shared expert of its own")
+            if shared_output.dtype != torch.bfloat16 or tuple(shared_output.shape) != (tokens, self.hidden) \
+                    or not shared_output.is_contiguous() or shared_output.device != self.device:
+                raise ValueError(f"shared_output must be contiguous bf16 [T, {self.hidden}] on {self.device}")
         b = {} if buffers is None else buffers
         dev = self.device
         if router_weight is not None:
@@ -422,6 +431,23 @@ class RoutedMoE:
         a.gamma = _ptr(gamma)
         a.norm_eps = 0.0 if comm is None else comm.eps
         a.residual_out = _ptr(res_out)
+        if shared_output is not None:
+            # the step up to the deferred rows, then the combine with the given shared rows
+            a.out = a.partial = a.comm = a.residual = a.gamma = a.residual_out = None
+            check(lib().mm_layer_forward(self._handle, ctypes.byref(a), _stream(dev)), "mm_layer_forward")
+            triple = (rows.data_ptr(), weights.data_ptr(), permuted.data_ptr(), shared_output.data_ptr())
+            if residual is not None:
+                check(lib().mm_finalize_allreduce_norm(comm.handle, *triple, residual.data_ptr(), _ptr(gamma), comm.eps,
+                                                       res_out.data_ptr(), _ptr(out), tokens, self.top_k, self.hidden,
+                                                       _stream(dev)), "mm_finalize_allreduce_norm")
+                return out, res_out
+            if comm is not None:
+                check(lib().mm_finalize_allreduce(comm.handle, *triple, out.data_ptr(), tokens, self.top_k, self.hidden,
+                                                  _stream(dev)), "mm_finalize_allreduce")
+            else:
+                check(lib().mm_finalize(*triple, _ptr(out), _ptr(part), tokens, self.top_k, self.hidden, _stream(dev)),
+                      "mm_finalize")
+            return part if partial else out
         check(lib().mm_layer_forward(self._handle, ctypes.byref(a), _stream(dev)), "mm_layer_forward")
         if residual is not None:
             return out, res_out
