@@ -52,6 +52,12 @@ __device__ __forceinline__ float int8_scale(uint32_t top) {
 // Scales below this (zero and NaN too) take int8_code_tiny.
 constexpr float kTinyScale = 0x1p-120f;
 
+// Whether two ranges of bytes share memory; null pointers do not.
+inline bool overlap(const void *p, int64_t p_bytes, const void *q, int64_t q_bytes) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return p && q && a < b + q_bytes && b < a + p_bytes;
+}
+
 // int8 codes and fp32 scales of rows (mm_norm.cu); returns an MM_* status.
 int quantize_rows(const char *what, const void *x, int64_t ld_x, int dtype, int8_t *codes, int64_t ld_codes,
                   float *scales, int tokens, int hidden, void *stream);

@@ -36,7 +36,7 @@ namespace mm {
 namespace {
 
 constexpr int kBlockK = 128;          // depth of a stage, bytes
-constexpr int kRowsM = 128;           // weight rows of a box, token rows of a pair's half
+constexpr int kRowsM = 128;           // the MMA's rows of a CTA: weight rows, or a pair's half of tokens
 constexpr int kBoxBytes = kRowsM * kBlockK;
 
 // Above this many tokens the tile form takes over.
@@ -56,7 +56,6 @@ struct alignas(64) Int8Args {
   int out_type;
   int stage_out;        // output rows start and end on 16-byte boundaries: TMA stores (a store
                         // that ends inside a 16-byte unit also writes the rest of the unit)
-  int gated;
   int has_clamp;
   float clamp;
   int token_tiles, feature_tiles, tile_n;  // of the tile form
@@ -471,6 +470,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0) {
+      pdl_wait();  // the loads start then: the bounded waits below count from there
       const uint32_t idesc = idesc_i8(kTileM, p.tile_n);
       int it = 0, n = 0;
       bool ok = true;
@@ -626,8 +626,8 @@ int encoder(EncodeFn *fn) {
   return MM_OK;
 }
 
-// Boxes of 128 (or 64) bytes by `box_rows` rows with the swizzle of that width; out-of-range elements read as zero
-// and are not written, so odd depths, tokens and features need no padding.
+// Boxes of 128 (or 64) bytes by `box_rows` rows with the swizzle of that width; out-of-range
+// elements read as zero and are not written, so odd depths, tokens and features need no padding.
 int encode(CUtensorMap *map, CUtensorMapDataType type, int es, const void *base, int64_t cols, int64_t rows_total,
            int64_t planes, int64_t ld, int box_rows, int box_bytes = 128) {
   EncodeFn fn;
@@ -760,11 +760,16 @@ int check(const char *what, const Product &q) {
     return set_error(MM_ERR_INVALID, "%s: int8 rows must start on 16-byte boundaries", what);
   if (!aligned(q.x_scale, 4) || !aligned(q.w_scale, 4) || !aligned(q.bias, 4) || !aligned(q.out, q.out_type == MM_DTYPE_FP32 ? 4 : 2))
     return set_error(MM_ERR_INVALID, "%s: a misaligned pointer", what);
+  const int es = q.out_type == MM_DTYPE_FP32 ? 4 : 2;
+  const int64_t w_rows = q.gated ? 2 * static_cast<int64_t>(q.features) : q.features;
+  if (overlap(q.out, ((q.tokens - 1) * q.ld_out + q.features) * es, q.x, (q.tokens - 1) * q.ld_x + q.depth) ||
+      overlap(q.out, ((q.tokens - 1) * q.ld_out + q.features) * es, q.w, (w_rows - 1) * q.ld_w + q.depth))
+    return set_error(MM_ERR_INVALID, "%s: the output overlaps an input", what);
   return MM_OK;
 }
 
 int run(const char *what, const Product &q, void *stream) {
-  Int8Args a;
+  Int8Args a = {};
   a.x_scale = q.x_scale;
   a.w_scale = q.w_scale;
   a.bias = q.bias;
@@ -774,7 +779,6 @@ int run(const char *what, const Product &q, void *stream) {
   a.features = q.features;
   a.blocks_k = (q.depth + kBlockK - 1) / kBlockK;
   a.out_type = q.out_type;
-  a.gated = q.gated;
   a.has_clamp = q.clamp > 0.0f;
   a.clamp = q.clamp;
   a.w_early = q.w_early;

@@ -716,18 +716,6 @@ cudaError_t launch_norm(const NormArgs &a, int quant, bool wide, void *stream) {
 
 int dtype_bytes(int dtype) { return dtype == MM_DTYPE_FP32 ? 4 : 2; }
 
-// Rows of a buffer, and whether two of them share memory.
-struct Span {
-  const void *p;
-  int64_t ld;
-};
-bool overlap(const Span &u, const Span &v, int tokens, int hidden, int es) {
-  if (!u.p || !v.p) return false;
-  const auto lo = [](const Span &s) { return reinterpret_cast<uintptr_t>(s.p); };
-  const auto hi = [&](const Span &s) { return lo(s) + ((tokens - 1) * s.ld + hidden) * es; };
-  return lo(u) < hi(v) && lo(v) < hi(u);
-}
-
 // Checks the sizes and picks the kernel's form: 16-byte chunks where x, the residual and the
 // outputs of x's type put each row at the same offset from a 16-byte boundary (MXFP8: at a
 // boundary, so that blocks and chunks agree), elements otherwise.
@@ -750,14 +738,15 @@ int run_norm(const char *what, NormArgs a, int dtype, int quant, void *stream) {
     return set_error(MM_ERR_INVALID, "%s: rows overlap (a row stride below %d)", what, a.hidden);
   const int es = dtype_bytes(dtype);
   // each thread writes the residual over elements that it alone has read, so that it may take
-  // x's or the residual's own place, row for row; nothing else may overlap an input
-  const Span in[] = {{a.x, a.ld_x}, {a.residual, a.ld_residual}};
-  for (const Span &s : in) {
-    if (overlap(s, {a.norm_out, a.ld_norm}, a.tokens, a.hidden, es) ||
-        (overlap(s, {a.residual_out, a.ld_residual_out}, a.tokens, a.hidden, es) &&
-         !(s.p == a.residual_out && s.ld == a.ld_residual_out)))
-      return set_error(MM_ERR_INVALID, "%s: an output overlaps an input", what);
-  }
+  // x's or the residual's own place, row for row; no other buffers may overlap
+  auto bytes = [&](int64_t ld) { return ((a.tokens - 1) * ld + a.hidden) * es; };
+  auto clash = [&](const void *p, int64_t ld_p, const void *q, int64_t ld_q) { return overlap(p, bytes(ld_p), q, bytes(ld_q)); };
+  auto moved = [&](const void *in, int64_t ld) {
+    return clash(in, ld, a.residual_out, a.ld_residual_out) && !(in == a.residual_out && ld == a.ld_residual_out);
+  };
+  if (clash(a.x, a.ld_x, a.norm_out, a.ld_norm) || clash(a.residual, a.ld_residual, a.norm_out, a.ld_norm) ||
+      clash(a.residual_out, a.ld_residual_out, a.norm_out, a.ld_norm) || moved(a.x, a.ld_x) || moved(a.residual, a.ld_residual))
+    return set_error(MM_ERR_INVALID, "%s: an output overlaps another buffer", what);
   const uintptr_t base = reinterpret_cast<uintptr_t>(a.x);
   bool wide = true;
   auto same = [&](const void *p, int64_t ld) {

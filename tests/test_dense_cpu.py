@@ -2,12 +2,14 @@
 ValueError (Python) before anything reaches the device, and empty calls launch nothing."""
 
 import ctypes
+import os
 
 import pytest
 import torch
 
 import megamoe
 from megamoe import _lib
+from test_kernel_resources import NVCC, _ptxas_info
 
 BUF = (ctypes.c_uint8 * (1 << 16))()
 BASE = (ctypes.addressof(BUF) + 255) & ~255  # a 256-byte aligned host address that is never read
@@ -52,6 +54,7 @@ def norm_args(**kw):
     (dict(norm_out=BASE + 20480 + 64), b"overlaps"),
     (dict(residual_out=BASE + 2), b"overlaps"),
     (dict(residual_out=BASE, ld_residual_out=128), b"overlaps"),
+    (dict(norm_out=BASE + 24576), b"overlaps"),
 ])
 def test_norm_refusals(bad, word):
     L = _lib.lib()
@@ -69,7 +72,7 @@ def test_empty_calls_launch_nothing():
 
 
 def linear(**kw):
-    a = dict(x=BASE, ld_x=64, xs=BASE, w=BASE, ld_w=64, ws=BASE, bias=None, out=BASE, ld_out=32, dtype=0, tokens=2,
+    a = dict(x=BASE, ld_x=64, xs=BASE, w=BASE + 8192, ld_w=64, ws=BASE, bias=None, out=BASE + 16384, ld_out=32, dtype=0, tokens=2,
              features=32, depth=64)
     a.update(kw)
     return _lib.lib().mm_int8_linear(a["x"], a["ld_x"], a["xs"], a["w"], a["ld_w"], a["ws"], a["bias"], a["out"],
@@ -79,9 +82,10 @@ def linear(**kw):
 @pytest.mark.parametrize("bad,status", [
     (dict(x=None), 1), (dict(xs=None), 1), (dict(w=None), 1), (dict(ws=None), 1), (dict(out=None), 1),
     (dict(x=BASE + 8), 1), (dict(w=BASE + 8), 1), (dict(ld_x=72), 1), (dict(ld_w=72), 1),
-    (dict(ld_x=48), 1), (dict(ld_w=48), 1), (dict(ld_out=31), 1), (dict(out=BASE + 1), 1),
+    (dict(ld_x=48), 1), (dict(ld_w=48), 1), (dict(ld_out=31), 1), (dict(out=BASE + 16385), 1),
     (dict(out=BASE + 2, dtype=2), 1), (dict(xs=BASE + 2), 1), (dict(bias=BASE + 2), 1), (dict(dtype=5), 1),
     (dict(tokens=-1), 1), (dict(features=0), 1), (dict(depth=0), 1),
+    (dict(out=BASE + 126), 1), (dict(out=BASE + 8192 + 2046), 1), (dict(out=BASE + 8192 - 126), 1),
     (dict(depth=1 << 17, ld_x=1 << 17, ld_w=1 << 17), 2), (dict(tokens=1 << 23), 2),
 ])
 def test_linear_refusals(bad, status):
@@ -91,8 +95,8 @@ def test_linear_refusals(bad, status):
 
 def ffn_args(**kw):
     a = _lib.MMInt8FFNArgs()
-    for f in ("x", "x_scale", "w13", "w13_scale", "w2", "w2_scale", "out", "workspace"):
-        setattr(a, f, BASE)
+    for i, f in enumerate(("x", "x_scale", "w13", "w13_scale", "w2", "w2_scale", "out", "workspace")):
+        setattr(a, f, BASE + 4096 * i)
     a.ld_x = a.ld_w13 = a.ld_out = 64
     a.ld_w2 = 32
     a.tokens, a.hidden, a.inter, a.out_dtype = 2, 64, 32, 0
@@ -132,6 +136,19 @@ def test_there_is_no_cpu_path():
         megamoe.int8_linear(q, s, q, s)
     with pytest.raises(ValueError, match="CUDA"):
         megamoe.int8_ffn(q, s, q, s, q, s)
+
+
+@pytest.mark.skipif(not os.path.exists(NVCC), reason="nvcc not found")
+@pytest.mark.parametrize("source,spills", [("mm_int8.cu", {}), ("mm_norm.cu", {"norm_rows_kernelIfLi8ELi2ELb0EE": 300})])
+def test_no_kernel_spills(source, spills):
+    """Only the fp32 row form that keeps two CTAs on an SM trades a few registers for them."""
+    kernels = _ptxas_info(source)
+    assert len(kernels) >= 8
+    for name, info in kernels.items():
+        most = next((v for k, v in spills.items() if k in name), 0)
+        assert info.get("spill", 0) <= most, (name, info)
+        if "int8_stream_kernel" in name:  # two CTAs an SM
+            assert info["regs"] <= 128
 
 
 def test_workspace_size():

@@ -15,6 +15,9 @@ Tolerances, from the arithmetic (u = 2^-24, fp32's half step; e = eps / 2, the o
 """
 
 import math
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -469,6 +472,30 @@ def test_streams_and_graphs():
     ins[0].mul_(-1)
     graphs[0].replay()
     assert torch.equal(outs[0], step(-xs[0]))
+
+
+@pytest.mark.parametrize("tokens", [1, 64, 300])
+def test_first_call_of_a_process_is_captured(tokens):
+    """Nothing that a first call sets up is closed to a capture."""
+    code = f"""
+import torch, megamoe
+x, g = torch.randn(({tokens}, 512), device="cuda").bfloat16(), torch.ones(512, device="cuda").bfloat16()
+w13, w2 = (torch.randint(-127, 127, s, dtype=torch.int8, device="cuda") for s in ((1024, 512), (512, 512)))
+s13, s2 = torch.full((1024,), 1e-3, device="cuda"), torch.full((512,), 1e-3, device="cuda")
+def step():
+    n = megamoe.rms_norm(x, g, quant="int8")
+    return megamoe.int8_ffn(n.codes, n.scales, w13, s13, w2, s2)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = step()
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(y, step()) and y.isfinite().all()
+"""
+    path = os.pathsep.join(p for p in sys.path if p)
+    done = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, PYTHONPATH=path), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
 
 
 def test_back_to_back_chain_reads_finished_inputs():
