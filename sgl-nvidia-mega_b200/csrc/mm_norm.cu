@@ -313,18 +313,21 @@ __device__ __forceinline__ uint4 gamma_chunk(const NormArgs &a, int e0) {
   return e0 < a.hidden ? C::load(p, e0, a.hidden, false) : make_uint4(0u, 0u, 0u, 0u);
 }
 
-// One CTA per row, NV chunks of it a thread, held in registers. Four and more take more than
+// One CTA per row, NV chunks of it a thread, held in registers. TURN: the int8 codes of rows
+// that start inside a 16-byte unit of x, while the codes' rows start on one, are turned in
+// shared memory (int8 rows of 1021 x 6147 by bytes 10.8 us, so 5.8). Four and more take more than
 // the 64 registers that 1024 threads leave each.
 // CTAs that shall share an SM: two of fp32 rows (h of a wide layer, 4096 x 18432: 70 us instead
 // of 92; 16-bit rows lose by it, 8192 x 7168 36 instead of 30), one of the latency form.
 constexpr int row_ctas(int nv, bool norm, int es) { return nv == 8 && !norm && es == 4 ? 2 : nv == 1 ? 1 : 0; }
 constexpr int row_threads(int nv, bool norm) { return nv >= 8 && norm ? 512 : nv >= 4 ? 640 : 1024; }
-template <typename T, int NV, int QUANT, bool NORM>
+template <typename T, int NV, int QUANT, bool NORM, bool TURN>
 __global__ void __launch_bounds__(row_threads(NV, NORM), row_ctas(NV, NORM, sizeof(T))) norm_rows_kernel(const __grid_constant__ NormArgs a) {
   using C = Chunk<T>;
   constexpr int VEC = C::kVec, PAIRS = C::kPairs;
   __shared__ double red_d[32];
   __shared__ uint32_t red_u[32], red_v[32];
+  extern __shared__ __align__(16) uint8_t code_row[];
   pdl_launch_dependents();
   pdl_wait();
   const int64_t t = blockIdx.x;
@@ -515,7 +518,35 @@ __global__ void __launch_bounds__(row_threads(NV, NORM), row_ctas(NV, NORM, size
       uint32_t w[VEC / 4];
 #pragma unroll
       for (int i = 0; i < VEC / 4; ++i) w[i] = pack4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
-      store_codes<VEC>(codes, e0, n, w, a.codes_wide && shift == 0 && e0 + VEC <= n);
+      if constexpr (TURN) {
+        uint8_t *to = code_row + (threadIdx.x + j * blockDim.x) * VEC;
+        if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[VEC / 4 - 1]);
+        else *reinterpret_cast<uint32_t *>(to) = w[0];
+      } else {
+        store_codes<VEC>(codes, e0, n, w, a.codes_wide && shift == 0 && e0 + VEC <= n);
+      }
+    }
+    if constexpr (TURN) {
+      // code e of the row sits at byte e + shift: 16-byte units of the row, shifted out of two
+      __syncthreads();
+      for (int u = threadIdx.x * 16; u < n; u += blockDim.x * 16) {
+        const uint4 lo = *reinterpret_cast<const uint4 *>(code_row + u), hi = *reinterpret_cast<const uint4 *>(code_row + u + 16);
+        uint32_t w[6] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y};
+        if (shift & 4) {
+#pragma unroll
+          for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+        }
+        const int bits = (shift & 3) * 8;
+        const uint32_t c[4] = {__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                               __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits)};
+        if (u + 16 <= n) {
+          *reinterpret_cast<uint4 *>(codes + u) = make_uint4(c[0], c[1], c[2], c[3]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (u + i < n) codes[u + i] = static_cast<uint8_t>(c[i / 4] >> (8 * (i % 4)));
+        }
+      }
     }
   }
 }
@@ -674,19 +705,21 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
 // 7168: two 98, four 83 (6.4 TB/s), eight 101; of 4096 x 16384: four 94, eight 128; of 8192 x
 // 2048: one 28, two 26; of 1024 x 5120: two 8.3, four 10.5, eight 16.8. int8 rows alone hold
 // less beside the row: 4096 x 16384: four 42, eight 35; 8192 x 7168: two 41, four 33, eight 30.5.
-template <typename T, int QUANT, bool NORM>
+template <typename T, int QUANT, bool NORM, bool TURN>
 cudaError_t launch_rows(const NormArgs &a, int chunks, void *stream) {
+  const size_t smem = TURN ? (static_cast<size_t>(chunks) * (16 / sizeof(T)) + 32) / 16 * 16 + 16 : 0;
   const unsigned rows = static_cast<unsigned>(a.tokens);
   auto threads = [&](int nv) { return dim3(((chunks + nv - 1) / nv + 31) / 32 * 32); };
   int nv;
   if (a.tokens <= kFewRows) nv = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
   else if (!NORM) nv = chunks <= 256 ? 2 : chunks <= 512 ? 4 : 8;
   else nv = chunks <= (a.tokens <= 2048 ? 1024 : 512) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
+  auto go = [&](auto kernel, int n) { return launch(kernel, dim3(rows), threads(n), smem, stream, a); };
   switch (nv) {
-    case 1: return launch(norm_rows_kernel<T, 1, QUANT, NORM>, dim3(rows), threads(1), 0, stream, a);
-    case 2: return launch(norm_rows_kernel<T, 2, QUANT, NORM>, dim3(rows), threads(2), 0, stream, a);
-    case 4: return launch(norm_rows_kernel<T, 4, QUANT, NORM>, dim3(rows), threads(4), 0, stream, a);
-    default: return launch(norm_rows_kernel<T, 8, QUANT, NORM>, dim3(rows), threads(8), 0, stream, a);
+    case 1: return go(norm_rows_kernel<T, 1, QUANT, NORM, TURN>, 1);
+    case 2: return go(norm_rows_kernel<T, 2, QUANT, NORM, TURN>, 2);
+    case 4: return go(norm_rows_kernel<T, 4, QUANT, NORM, TURN>, 4);
+    default: return go(norm_rows_kernel<T, 8, QUANT, NORM, TURN>, 8);
   }
 }
 
@@ -700,9 +733,12 @@ cudaError_t launch_norm(const NormArgs &a, bool wide, void *stream) {
   const bool shifted = (reinterpret_cast<uintptr_t>(a.x) % 16) || (a.ld_x * static_cast<int64_t>(sizeof(T))) % 16;
   const int chunks = (a.hidden + VEC - 1) / VEC + (shifted ? 1 : 0);
   if (chunks > 8 * row_threads(8, a.gamma != nullptr)) return launch(norm_kernel<T, VEC, QUANT>, dim3(rows), dim3(1024), 0, stream, a);
-  if constexpr (QUANT == MM_QUANT_INT8)
-    if (!a.gamma) return launch_rows<T, QUANT, false>(a, chunks, stream);
-  return launch_rows<T, QUANT, true>(a, chunks, stream);
+  if constexpr (QUANT == MM_QUANT_INT8) {
+    if (!a.gamma)
+      return a.code_row ? launch_rows<T, QUANT, false, true>(a, chunks, stream) : launch_rows<T, QUANT, false, false>(a, chunks, stream);
+    if (a.code_row) return launch_rows<T, QUANT, true, true>(a, chunks, stream);
+  }
+  return launch_rows<T, QUANT, true, false>(a, chunks, stream);
 }
 
 template <typename T>
@@ -761,6 +797,7 @@ int run_norm(const char *what, NormArgs a, int dtype, int quant, void *stream) {
   wide = same(a.residual, a.ld_residual) && same(a.residual_out, a.ld_residual_out) && same(a.norm_out, a.ld_norm);
   const bool shifted = base % 16 || a.ld_x * es % 16;
   a.codes_wide = quant && reinterpret_cast<uintptr_t>(a.codes) % 8 == 0 && a.ld_codes % 8 == 0;
+  a.code_row = quant == MM_QUANT_INT8 && shifted && reinterpret_cast<uintptr_t>(a.codes) % 16 == 0 && a.ld_codes % 16 == 0;
   if (quant == MM_QUANT_MXFP8 && (shifted || !a.codes_wide)) wide = false;
   a.gamma_wide = a.gamma && reinterpret_cast<uintptr_t>(a.gamma) % 16 == 0;
   cudaError_t e;

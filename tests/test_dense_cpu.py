@@ -139,7 +139,7 @@ def test_there_is_no_cpu_path():
 
 
 @pytest.mark.skipif(not os.path.exists(NVCC), reason="nvcc not found")
-@pytest.mark.parametrize("source,spills", [("mm_int8.cu", {}), ("mm_norm.cu", {"norm_rows_kernelIfLi8ELi2ELb0EE": 300})])
+@pytest.mark.parametrize("source,spills", [("mm_int8.cu", {}), ("mm_norm.cu", {"norm_rows_kernelIfLi8ELi2ELb0E": 300})])
 def test_no_kernel_spills(source, spills):
     """Only the fp32 row form that keeps two CTAs on an SM trades a few registers for them."""
     kernels = _ptxas_info(source)
