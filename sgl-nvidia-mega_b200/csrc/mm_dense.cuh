@@ -9,6 +9,8 @@ namespace mm {
 // Up to this many rows a row kernel spreads each over as many threads as it has 16-byte
 // chunks; beyond, rows share the SMs.
 constexpr int kFewRows = 296;
+// Short rows share CTAs from this many on (four CTAs an SM at four rows each).
+constexpr int kShareRows = 4 * 592;
 
 struct NormArgs {
   const void *x;             // [tokens, hidden], row stride ld_x (elements)
@@ -25,6 +27,7 @@ struct NormArgs {
   int gamma_f32;             // gamma is fp32 beside a 16-bit x
   int gamma_wide;            // gamma starts on a 16-byte boundary
   int codes_wide;            // code rows start on 8-byte boundaries
+  int turn_bytes;            // shared memory of a row of them
   int code_row;              // int8 codes on 16-byte boundaries of rows that are not
 };
 

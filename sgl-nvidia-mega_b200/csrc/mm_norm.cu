@@ -327,10 +327,12 @@ __global__ void __launch_bounds__(row_threads(NV, NORM), row_ctas(NV, NORM, size
   constexpr int VEC = C::kVec, PAIRS = C::kPairs;
   __shared__ double red_d[32];
   __shared__ uint32_t red_u[32], red_v[32];
-  extern __shared__ __align__(16) uint8_t code_row[];
+  extern __shared__ __align__(16) uint8_t code_rows[];
+  uint8_t *turned = code_rows + threadIdx.y * a.turn_bytes;
   pdl_launch_dependents();
   pdl_wait();
-  const int64_t t = blockIdx.x;
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  if (t >= a.tokens) return;  // rows share a CTA only where a warp has each
   const int n = a.hidden;
   const T *x = static_cast<const T *>(a.x) + t * a.ld_x;
   const T *res = NORM && a.residual ? static_cast<const T *>(a.residual) + t * a.ld_residual : nullptr;
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(row_threads(NV, NORM), row_ctas(NV, NORM, size
 #pragma unroll
       for (int i = 0; i < VEC / 4; ++i) w[i] = pack4(q[4 * i], q[4 * i + 1], q[4 * i + 2], q[4 * i + 3]);
       if constexpr (TURN) {
-        uint8_t *to = code_row + (threadIdx.x + j * blockDim.x) * VEC;
+        uint8_t *to = turned + (threadIdx.x + j * blockDim.x) * VEC;
         if constexpr (VEC == 8) *reinterpret_cast<uint2 *>(to) = make_uint2(w[0], w[VEC / 4 - 1]);
         else *reinterpret_cast<uint32_t *>(to) = w[0];
       } else {
@@ -528,9 +530,10 @@ __global__ void __launch_bounds__(row_threads(NV, NORM), row_ctas(NV, NORM, size
     }
     if constexpr (TURN) {
       // code e of the row sits at byte e + shift: 16-byte units of the row, shifted out of two
-      __syncthreads();
+      if (blockDim.x == 32) __syncwarp();
+      else __syncthreads();
       for (int u = threadIdx.x * 16; u < n; u += blockDim.x * 16) {
-        const uint4 lo = *reinterpret_cast<const uint4 *>(code_row + u), hi = *reinterpret_cast<const uint4 *>(code_row + u + 16);
+        const uint4 lo = *reinterpret_cast<const uint4 *>(turned + u), hi = *reinterpret_cast<const uint4 *>(turned + u + 16);
         uint32_t w[6] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y};
         if (shift & 4) {
 #pragma unroll
@@ -706,15 +709,20 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
 // 2048: one 28, two 26; of 1024 x 5120: two 8.3, four 10.5, eight 16.8. int8 rows alone hold
 // less beside the row: 4096 x 16384: four 42, eight 35; 8192 x 7168: two 41, four 33, eight 30.5.
 template <typename T, int QUANT, bool NORM, bool TURN>
-cudaError_t launch_rows(const NormArgs &a, int chunks, void *stream) {
-  const size_t smem = TURN ? (static_cast<size_t>(chunks) * (16 / sizeof(T)) + 32) / 16 * 16 + 16 : 0;
-  const unsigned rows = static_cast<unsigned>(a.tokens);
-  auto threads = [&](int nv) { return dim3(((chunks + nv - 1) / nv + 31) / 32 * 32); };
+cudaError_t launch_rows(NormArgs a, int chunks, void *stream) {
+  a.turn_bytes = TURN ? static_cast<int>((chunks * (16 / sizeof(T)) + 32) / 16 * 16 + 16) : 0;
+  // Short rows in number share CTAs, a warp each (int8 rows of 8192 x 1024 5.4 us instead of 9.2,
+  // norm of 8192 x 512 6.1 instead of 9.4; norm with int8 of 1300 x 1024 6.0 instead of 4.4).
+  const int share = chunks > 128 || a.tokens < kShareRows ? 1 : a.tokens < 2 * kShareRows ? 4 : 8;
   int nv;
-  if (a.tokens <= kFewRows) nv = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
+  if (share > 1) nv = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
+  else if (a.tokens <= kFewRows) nv = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
   else if (!NORM) nv = chunks <= 256 ? 2 : chunks <= 512 ? 4 : 8;
   else nv = chunks <= (a.tokens <= 2048 ? 1024 : 512) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
-  auto go = [&](auto kernel, int n) { return launch(kernel, dim3(rows), threads(n), smem, stream, a); };
+  auto go = [&](auto kernel, int n) {
+    const dim3 block = share > 1 ? dim3(32, share) : dim3(((chunks + n - 1) / n + 31) / 32 * 32);
+    return launch(kernel, dim3((a.tokens + share - 1) / share), block, share * a.turn_bytes, stream, a);
+  };
   switch (nv) {
     case 1: return go(norm_rows_kernel<T, 1, QUANT, NORM, TURN>, 1);
     case 2: return go(norm_rows_kernel<T, 2, QUANT, NORM, TURN>, 2);

@@ -96,7 +96,7 @@ def check_norm(got, x, gamma, eps, residual, quant, with_norm):
 @pytest.mark.parametrize("quant", [None, "mxfp8", "int8"])
 @pytest.mark.parametrize("tokens,hidden,residual", [
     (1, 7168, True), (1, 32, False), (3, 1024, True), (48, 5120, False), (297, 6144, True), (300, 96, True),
-    (2, 16384, True), (300, 16384, False), (2, 40000, True), (300, 40032, False),
+    (2, 16384, True), (300, 16384, False), (2, 40000, True), (300, 40032, False), (2501, 512, True), (4801, 1024, True),
 ])
 def test_norm(tokens, hidden, residual, quant, dtype):
     if quant == "mxfp8":
@@ -112,7 +112,7 @@ def test_norm(tokens, hidden, residual, quant, dtype):
 
 @pytest.mark.parametrize("dtype", [BF, FH, F32])
 @pytest.mark.parametrize("quant", [None, "int8"])
-@pytest.mark.parametrize("tokens,hidden", [(1, 1), (2, 7), (5, 33), (3, 1001), (299, 4099), (2, 16383), (1, 50001)])
+@pytest.mark.parametrize("tokens,hidden", [(1, 1), (2, 7), (5, 33), (3, 1001), (299, 4099), (2, 16383), (1, 50001), (2499, 505), (4803, 1017)])
 def test_norm_odd_rows(tokens, hidden, quant, dtype):
     g = gen(tokens, hidden, 5)
     x, res = randn((tokens, hidden), g, dtype), randn((tokens, hidden), g, dtype)
@@ -184,7 +184,7 @@ def test_norm_zero_row_and_zero_eps():
 
 
 @pytest.mark.parametrize("dtype", [BF, FH, F32])
-@pytest.mark.parametrize("tokens,hidden", [(1, 1), (1, 7168), (8, 7168), (3, 1001), (300, 2048), (301, 999), (2, 18432), (5, 70001)])
+@pytest.mark.parametrize("tokens,hidden", [(1, 1), (1, 7168), (8, 7168), (3, 1001), (300, 2048), (301, 999), (2, 18432), (5, 70001), (5001, 1024), (2999, 77)])
 def test_quantize_bit_exact(tokens, hidden, dtype):
     g = gen(tokens, hidden, 3)
     x = (randn((tokens, hidden), g) * torch.exp(4 * randn((tokens, 1), g))).to(dtype)
