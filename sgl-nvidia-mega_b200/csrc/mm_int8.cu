@@ -39,8 +39,10 @@ constexpr int kBlockK = 128;          // depth of a stage, bytes
 constexpr int kRowsM = 128;           // the MMA's rows of a CTA: weight rows, or a pair's half of tokens
 constexpr int kBoxBytes = kRowsM * kBlockK;
 
-// Above this many tokens the tile form takes over.
+// Up to this many tokens the stream form always, beyond it what the estimates say (us).
 constexpr int kTileTokens = 128;
+constexpr double kTileUs = 4.0, kTileColumnUs = 0.346 / 448;  // a launch; a column of a block of depth
+constexpr double kStreamUs = 7.5, kStreamBlockUs = 0.45;      // a round of 128-token CTAs; a block
 
 // Error word of this file's launches: bounded waits that ran out (mm_int8_check).
 __device__ uint32_t g_int8_error;
@@ -147,6 +149,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   const int split = p.split;
   const int rank = split > 1 ? static_cast<int>(cluster_rank()) : 0;
   const int f0 = (blockIdx.x / split) * S::kFeatures;
+  const int t0 = blockIdx.y * BN, live = min(BN, p.tokens - t0);
   const int kb0 = p.blocks_k * rank / split, kb1 = p.blocks_k * (rank + 1) / split;
   const int n = kb1 - kb0;
 
@@ -167,7 +170,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     *failed = 0u;
     fence_barrier_init();
     // a part of each token that this CTA finishes, from every CTA
-    const int mine = (p.tokens - rank + split - 1) / split;
+    const int mine = (live - rank + split - 1) / split;
     if (S::kPush && split > 1 && mine > 0) mbar_expect_tx(recv, mine * split * kRowsM * 4);
   }
   if (warp == 1) {
@@ -195,7 +198,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       mbar_expect_tx(bar, S::kStageBytes);
 #pragma unroll
       for (int a = 0; a < kRowsM / S::kFeatures; ++a)
-        tma_load_3d(stage + a * S::kFeatures * kBlockK, &p.w_map, (kb0 + i) * kBlockK, f0, a, bar, stream_once);
+        tma_load_3d(stage + a * S::kFeatures * kBlockK, &p.w_map, (kb0 + i) * kBlockK, f0, a, bar, gridDim.y > 1 ? keep : stream_once);
     };
     const int early = p.w_early ? min(n, S::kStages) : 0;
     if (elect_one())
@@ -211,7 +214,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
         break;
       if (elect_one()) {
         if (i >= early) load_w(i);
-        tma_load_2d(ring + s * S::kStageBytes + kBoxBytes, &p.x_map, (kb0 + i) * kBlockK, 0, full + 8 * s, keep);
+        tma_load_2d(ring + s * S::kStageBytes + kBoxBytes, &p.x_map, (kb0 + i) * kBlockK, t0, full + 8 * s, keep);
       }
       __syncwarp();
     }
@@ -256,7 +259,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     ws[i] = i < left ? p.w_scale[f + i] : 0.0f;
     second[i] = i >= left ? 0.0f : GATED ? p.w_scale[static_cast<int64_t>(p.features) + f + i] : p.bias ? p.bias[f + i] : 0.0f;
   }
-  if (warp >= 2 && threadIdx.x - 64 < p.tokens) x_scale[threadIdx.x - 64] = p.x_scale[threadIdx.x - 64];
+  if (warp >= 2 && threadIdx.x - 64 < live) x_scale[threadIdx.x - 64] = p.x_scale[t0 + threadIdx.x - 64];
   bool ok = mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc);
   tc_fence_after();
   ok = ok && *failed == 0u;
@@ -274,7 +277,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       if constexpr (GATED) v[i] = gate_up(p, __fmul_rn(a[i], ws[i]), __fmul_rn(a[PER + i], second[i]));
       else v[i] = __fmaf_rn(a[i], ws[i], second[i]);
     }
-    if (ok && left > 0) store_some<PER>(p, j * p.ld_out + f, left, v, wide);
+    if (ok && left > 0) store_some<PER>(p, (t0 + j) * p.ld_out + f, left, v, wide);
   };
   // the four sums of a lane: four features, or two features' gate and up
   auto add = [](int4 &sum, const int4 &v) { sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w; };
@@ -286,7 +289,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       const int turns = __ffs(split) - 1;  // split is a power of two
       const uint32_t at = ring + (rank * kRowsM + q * 32 + lane) * 4;
 #pragma unroll 1
-      for (int j = 0; j < p.tokens; j += 16) {
+      for (int j = 0; j < live; j += 16) {
         uint32_t r[16];
         tc_ld_32x32b_x16(sums + j, r);
         tc_wait_ld();
@@ -294,7 +297,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int owner = (j + i) & (split - 1), turn = (j + i) >> turns;
-          if (j + i < p.tokens)
+          if (j + i < live)
             cluster_store_async(cluster_map(at + turn * split * kRowsM * 4, owner), r[i], cluster_map(recv, owner));
         }
       }
@@ -304,12 +307,12 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     tc_fence_before();
     __syncthreads();  // x's scales, and the TMEM reads
     if (warp == 1) tmem_dealloc(tmem, S::kCols);
-    if (rank < p.tokens && !mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc)) {
+    if (rank < live && !mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc)) {
       cluster_sync();  // parts may still come: stay until their senders are gone
       return;
     }
 #pragma unroll 1
-    for (int j = rank + split * warp; j < p.tokens; j += split * kStreamWarps) {
+    for (int j = rank + split * warp; j < live; j += split * kStreamWarps) {
       const int *part = reinterpret_cast<const int *>(ring_ptr) + (j & ~(split - 1)) * kRowsM + PER * lane;
       int4 sum = make_int4(0, 0, 0, 0);
 #pragma unroll 8
@@ -328,7 +331,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   // Each CTA leaves its parts in its own ring, [token][weight row], and reads the others' there.
   if (warp >= 2) {
 #pragma unroll 1
-    for (int j = 0; j < p.tokens; j += 16) {
+    for (int j = 0; j < live; j += 16) {
       uint32_t r[16];
       tc_ld_32x32b_x16(sums + j, r);
       tc_wait_ld();
@@ -341,7 +344,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   cluster_sync();
   if (warp == 1) tmem_dealloc(tmem, S::kCols);
 #pragma unroll 1
-  for (int j = rank + split * warp; j < p.tokens; j += split * kStreamWarps) {
+  for (int j = rank + split * warp; j < live; j += split * kStreamWarps) {
     const uint32_t at = ring + (j * kRowsM + PER * lane) * 4;
     int4 sum = make_int4(0, 0, 0, 0);
 #pragma unroll 4
@@ -361,7 +364,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
 
 // ---------------------------------------------------------------------------------------
 // The tile form. Per CTA: warp 0 loads, warp 1 (of the pair's leader) issues the products,
-// warps 2..5 are the epilogue; every warp of both CTAs walks the same tiles.
+// warps 2..9 are the epilogue; every warp of both CTAs walks the same tiles.
 constexpr int kTileM = 256;                        // tokens of a pair
 constexpr int kTileN = 256;                        // weight rows of a pair at most
 // A stage is two blocks of depth, 64 KB of this CTA's halves of both operands: a hand-over
@@ -371,10 +374,13 @@ constexpr int kTileN = 256;                        // weight rows of a pair at m
 constexpr int kTileBlocks = 2;
 constexpr int kTileStages = 3;
 constexpr int kTileStageBytes = kTileBlocks * 2 * kBoxBytes;
-constexpr int kTileThreads = 192;
-constexpr int kOutChunk = 32;                      // columns of one TMEM read and one store
-constexpr int kOutBytes = 32 * kOutChunk * 4;      // a warp's staged chunk (32 rows), fp32
-constexpr int kTileSmem = 1024 + kTileStages * kTileStageBytes + 4 * kOutBytes + 4 * 2 * kTileN * 4 + 256;
+// Eight epilogue warps: two a quarter of the TMEM lanes take turns by chunks of columns (with
+// four, 4096 x 7008 x 512 was bound by them: 34 us).
+constexpr int kEpilogueWarps = 8;
+constexpr int kTileThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kOutBytes = 32 * 64;                 // a staged chunk: 32 rows of 64 bytes
+constexpr int kScaleFloats = 2 * (kTileN / 2);     // a warp's columns' scales, and bias or up scales
+constexpr int kTileSmem = 1024 + kTileStages * kTileStageBytes + kEpilogueWarps * (kOutBytes + kScaleFloats * 4) + 256;
 
 // The tile of a step: token tiles in groups of 16 (their codes stay in L2 while the weights
 // pass by once a group), fastest inside a group.
@@ -393,8 +399,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
   const uint32_t ring = (raw + 1023u) & ~1023u;
   uint8_t *base = smem_raw + (ring - raw);
   const uint32_t out_stage = ring + kTileStages * kTileStageBytes;
-  float *scales = reinterpret_cast<float *>(base + kTileStages * kTileStageBytes + 4 * kOutBytes);
-  const uint32_t bars = out_stage + 4 * kOutBytes + 4 * 2 * kTileN * 4;
+  float *scales = reinterpret_cast<float *>(base + kTileStages * kTileStageBytes + kEpilogueWarps * kOutBytes);
+  const uint32_t bars = out_stage + kEpilogueWarps * (kOutBytes + kScaleFloats * 4);
   const uint32_t full = bars, empty = full + 8 * kTileStages, acc_full = empty + 8 * kTileStages,
                  acc_empty = acc_full + 16, drained = acc_empty + 16, slot = drained + 8;
   uint32_t *slot_ptr = reinterpret_cast<uint32_t *>(base + (slot - ring));
@@ -416,7 +422,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(acc_full + 8 * b, 1);
-      mbar_init(acc_empty + 8 * b, 8);  // four epilogue warps of either CTA
+      mbar_init(acc_empty + 8 * b, 2 * kEpilogueWarps);  // of both CTAs
     }
     mbar_init(drained, 1);
     fence_barrier_init();
@@ -429,10 +435,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *slot_ptr;
-  pdl_launch_dependents();  // after the allocation, as in the stream form
+  // after the allocation and the wait, as in the stream form; the bounded waits below count from here
+  pdl_wait();
+  pdl_launch_dependents();
 
   if (warp == 0) {
-    pdl_wait();
     const uint32_t block_tx = 2 * (kBoxBytes + half_n * kBlockK);  // both CTAs' bytes
     int it = 0;
     bool ok = true;
@@ -470,7 +477,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0) {
-      pdl_wait();  // the loads start then: the bounded waits below count from there
       const uint32_t idesc = idesc_i8(kTileM, p.tile_n);
       int it = 0, n = 0;
       bool ok = true;
@@ -508,10 +514,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
     }
     __syncwarp();
   } else {
-    pdl_wait();
-    const int q = warp & 3;  // TMEM lanes 32 q and on: token rows
-    float *ws = scales + q * 2 * kTileN, *second = ws + kTileN;  // second: the bias, or the up rows' scales
-    const uint32_t mine = out_stage + q * kOutBytes;
+    constexpr int CH = 64 / sizeof(Out);           // columns of a chunk
+    const int q = warp & 3, e = warp - 2;          // TMEM lanes 32 q and on: token rows
+    const int half = e >> 2;                       // this warp's chunks: half, half + 2, ...
+    float *ws = scales + e * kScaleFloats, *second = ws + kScaleFloats / 2;  // second: the bias, or the up rows' scales
+    const uint32_t mine = out_stage + e * kOutBytes;
     int n = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++n) {
       const int b = n & 1;
@@ -521,30 +528,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       const int f0 = ft * tile_f;
       const float xs = t < p.tokens ? p.x_scale[t] : 0.0f;
       __syncwarp();
-      for (int i = lane; i < tile_f; i += 32) {
-        const bool in = f0 + i < p.features;
-        ws[i] = in ? p.w_scale[f0 + i] : 0.0f;
-        second[i] = !in ? 0.0f : GATED ? p.w_scale[p.features + f0 + i] : p.bias ? p.bias[f0 + i] : 0.0f;
+      for (int i = lane; i < tile_f / 2 + CH; i += 32) {
+        const int f = f0 + (2 * (i / CH) + half) * CH + i % CH;  // its place among this warp's chunks
+        const bool in = i < kScaleFloats / 2 && f < min(p.features, f0 + tile_f);
+        if (i < kScaleFloats / 2) {
+          ws[i] = in ? p.w_scale[f] : 0.0f;
+          second[i] = !in ? 0.0f : GATED ? p.w_scale[p.features + f] : p.bias ? p.bias[f] : 0.0f;
+        }
       }
       __syncwarp();
       if (!warp_agrees(mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc))) break;
       tc_fence_after();
       const uint32_t from = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kTileN;
-      for (int c = 0; c < tile_f; c += kOutChunk) {
-        uint32_t r[kOutChunk], u[GATED ? kOutChunk : 1];
-        tc_ld_32x32b_x32(from + c, r);
-        if constexpr (GATED) tc_ld_32x32b_x32(from + half_n + c, u);
+      for (int c = half * CH, i0 = 0; c < tile_f; c += 2 * CH, i0 += CH) {
+        uint32_t r[CH], u[GATED ? CH : 1];
+        if constexpr (CH == 32) tc_ld_32x32b_x32(from + c, r);
+        else tc_ld_32x32b_x16(from + c, r);
+        if constexpr (GATED) tc_ld_32x32b_x16(from + half_n + c, u);
         tc_wait_ld();
-        if (c + kOutChunk == tile_f) {
-          // the accumulator is in registers: the pair's next but one tile may overwrite it
+        if (c + 2 * CH >= tile_f) {
+          // this warp's columns are in registers: the pair's next but one tile may overwrite them
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(cluster_map(acc_empty + 8 * b, 0));
         }
-        float v[kOutChunk];
+        float v[CH];
 #pragma unroll
-        for (int j = 0; j < kOutChunk; j += 4) {
-          const float4 w4 = *reinterpret_cast<const float4 *>(ws + c + j), s4 = *reinterpret_cast<const float4 *>(second + c + j);
+        for (int j = 0; j < CH; j += 4) {
+          const float4 w4 = *reinterpret_cast<const float4 *>(ws + i0 + j), s4 = *reinterpret_cast<const float4 *>(second + i0 + j);
           const float w[4] = {w4.x, w4.y, w4.z, w4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -555,26 +566,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
               v[j + i] = __fmaf_rn(a, w[i], s[i]);
           }
         }
+        uint32_t word[16];  // the row's 64 bytes
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          if constexpr (sizeof(Out) == 4) {
+            word[i] = __float_as_uint(v[i]);
+          } else {
+            union { uint32_t w; Out h[2]; } pk;
+            pk.h[0] = Out(v[2 * i]);
+            pk.h[1] = Out(v[2 * i + 1]);
+            word[i] = pk.w;
+          }
+        }
+        uint8_t *buf = base + (mine - ring);
         if (p.stage_out) {
-          // this warp's [32 rows][32 columns], swizzled as the map says (16-byte units XORed
-          // with the row so that eight lanes' stores touch eight banks' units), then one store
+          // this warp's 32 rows, swizzled as the map says (16-byte units XORed with the row, so
+          // that eight lanes' stores meet no bank twice), then one store
           if (lane == 0) bulk_wait_read<0>();
           __syncwarp();
-          uint8_t *row = base + (mine - ring);
-          if constexpr (sizeof(Out) == 4) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              *reinterpret_cast<float4 *>(row + lane * 128 + ((i ^ (lane & 7)) * 16)) =
-                  make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              union { uint4 w; Out h[8]; } pk;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) pk.h[j] = Out(v[8 * i + j]);
-              *reinterpret_cast<uint4 *>(row + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)) = pk.w;
-            }
-          }
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4 *>(buf + lane * 64 + ((i ^ ((lane >> 1) & 3)) * 16)) =
+                make_uint4(word[4 * i], word[4 * i + 1], word[4 * i + 2], word[4 * i + 3]);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && t0 < p.tokens && f0 + c < p.features) {
@@ -582,17 +595,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
             bulk_commit_group();
           }
         } else {
-          // rows that TMA cannot store: turned in shared memory (columns XORed with the row: no
-          // bank meets twice), then a row of 32 columns an instruction
-          float *turn = reinterpret_cast<float *>(base + (mine - ring));
+          // rows that TMA cannot store: turned in shared memory (words XORed with the row), then
+          // whole rows an instruction, one of 16-bit columns or two of fp32
+          uint32_t *turn = reinterpret_cast<uint32_t *>(buf);
 #pragma unroll
-          for (int i = 0; i < kOutChunk; ++i) turn[lane * 32 + (i ^ lane)] = v[i];
+          for (int i = 0; i < 16; ++i) turn[lane * 16 + (i ^ (lane & 15))] = word[i];
           __syncwarp();
-          const int rows = min(32, p.tokens - t0);
-          if (f0 + c + lane < p.features) {
-            Out *o = static_cast<Out *>(p.out) + t0 * p.ld_out + f0 + c + lane;
+          constexpr int AT_ONCE = 32 / CH;
+          const int col = lane & (CH - 1), rows = min(32, p.tokens - t0);
+          if (f0 + c + col < p.features) {
+            Out *o = static_cast<Out *>(p.out) + static_cast<int64_t>(t0) * p.ld_out + f0 + c + col;
 #pragma unroll 8
-            for (int j = 0; j < rows; ++j, o += p.ld_out) *o = Out(turn[j * 32 + (lane ^ j)]);
+            for (int j = lane / CH; j < rows; j += AT_ONCE) {
+              const Out *at = reinterpret_cast<const Out *>(turn + j * 16 + ((col * static_cast<int>(sizeof(Out)) / 4) ^ (j & 15)));
+              o[j * p.ld_out] = at[sizeof(Out) == 4 ? 0 : col & 1];
+            }
           }
           __syncwarp();
         }
@@ -673,18 +690,23 @@ cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, int clust
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+// CTAs of a cluster that share a tile's depth: enough CTAs for most SMs, each with at least two
+// blocks of depth.
+int stream_split(int64_t tiles, int blocks_k) {
+  int split = 1;
+  while (split < 8 && tiles * split < 148 && 4 * split <= blocks_k) split *= 2;
+  return split;
+}
+
 template <int BN, bool GATED>
 cudaError_t launch_stream(Int8Args &a, void *stream) {
   using S = Stream<BN, GATED>;
   static bool done[64] = {};
   const cudaError_t e = raise_smem(int8_stream_kernel<BN, GATED>, S::kSmem, done);
   if (e != cudaSuccess) return e;
-  const int tiles = (a.features + S::kFeatures - 1) / S::kFeatures;
-  // enough CTAs for two an SM, each with at least two stages of depth
-  int split = 1;
-  while (split < 8 && tiles * split < 148 && 4 * split <= a.blocks_k) split *= 2;
-  a.split = split;
-  return launch_cluster(int8_stream_kernel<BN, GATED>, dim3(tiles * split), kStreamThreads, S::kSmem, split, stream, a);
+  const int tiles = (a.features + S::kFeatures - 1) / S::kFeatures, token_tiles = (a.tokens + BN - 1) / BN;
+  a.split = stream_split(tiles * token_tiles, a.blocks_k);
+  return launch_cluster(int8_stream_kernel<BN, GATED>, dim3(tiles * a.split, token_tiles), kStreamThreads, S::kSmem, a.split, stream, a);
 }
 
 // CTA pairs that the current device runs at once (of the tile form: one CTA an SM, all its
@@ -786,21 +808,24 @@ int run(const char *what, const Product &q, void *stream) {
   int rc;
   auto x_map = [&](int rows) { return encode(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, q.depth, q.tokens, 0, q.ld_x, rows); };
   cudaError_t e;
-  if (q.tokens > kTileTokens) {
-    const int pairs = sm_pairs();
-    if (pairs < 1) return set_error(MM_ERR_CUDA, "%s: the tile form does not fit this device", what);
-    // the width that leaves the pairs the least to do: a tile's time grows as its width plus
-    // 192 columns (8192 x 7168 x 7168, a tile's share of the whole: 19.4 us at 256 columns,
-    // 13.0 at 128, 11.1 at 64). 2048 tokens: 224 columns 72 us, 256 columns 74, 128 columns 87;
-    // 1024 x 2048 x 7168: 128 columns 16.1 us, 256 columns 23.1.
-    int64_t best = INT64_MAX;
-    a.token_tiles = (q.tokens + kTileM - 1) / kTileM;
-    for (int n = kTileN; n >= 64; n -= q.gated ? 64 : 32) {
-      const int f = q.gated ? n / 2 : n;
-      const int64_t tiles = static_cast<int64_t>(a.token_tiles) * ((q.features + f - 1) / f);
-      const int64_t cost = (tiles + pairs - 1) / pairs * (n + 192);
-      if (cost < best) best = cost, a.tile_n = n, a.feature_tiles = (q.features + f - 1) / f;
-    }
+  const int pairs = sm_pairs();
+  if (pairs < 1) return set_error(MM_ERR_CUDA, "%s: CTA pairs do not fit this device", what);
+  // Which form, and the tile form's width, by the time that they take. A tile's time grows with
+  // the depth and as its width plus 192 columns (8192 x 7168 x 7168, a tile's share of the whole:
+  // 19.4 us at 256 columns, 13.0 at 128, 11.1 at 64). 2048 tokens: 224 columns 72 us, 256 columns
+  // 74, 128 columns 87; 1024 x 2048 x 7168: 128 columns 16.1 us, 256 columns 23.1.
+  double tile_us = 1e30;
+  a.token_tiles = (q.tokens + kTileM - 1) / kTileM;
+  for (int n = kTileN; n >= 64; n -= q.gated ? 64 : 32) {
+    const int f = q.gated ? n / 2 : n;
+    const int64_t tiles = static_cast<int64_t>(a.token_tiles) * ((q.features + f - 1) / f);
+    const double us = kTileUs + static_cast<double>((tiles + pairs - 1) / pairs) * a.blocks_k * (n + 192) * kTileColumnUs;
+    if (us < tile_us) tile_us = us, a.tile_n = n, a.feature_tiles = (q.features + f - 1) / f;
+  }
+  const int64_t stream_tiles = (static_cast<int64_t>(q.features) * (q.gated ? 2 : 1) + kRowsM - 1) / kRowsM * ((q.tokens + 127) / 128);
+  const int split = stream_split(stream_tiles, a.blocks_k);
+  const double stream_us = static_cast<double>((stream_tiles * split + 295) / 296) * (kStreamUs + (a.blocks_k + split - 1) / split * kStreamBlockUs);
+  if (q.tokens > kTileTokens && (tile_us <= stream_us || q.tokens > 65535 * 128)) {
     const int es = q.out_type == MM_DTYPE_FP32 ? 4 : 2;
     a.stage_out = aligned(q.out, 16) && q.ld_out * es % 16 == 0 && (q.out_pad || static_cast<int64_t>(q.features) * es % 16 == 0);
     if ((rc = x_map(kRowsM)) || (rc = w_map(a.tile_n / 2))) return rc;
@@ -808,7 +833,7 @@ int run(const char *what, const Product &q, void *stream) {
         (rc = encode(&a.out_map, q.out_type == MM_DTYPE_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                  : q.out_type == MM_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
                                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                     es, q.out, q.features, q.tokens, 0, q.ld_out, 32, kOutChunk * es)))
+                     es, q.out, q.features, q.tokens, 0, q.ld_out, 32, 64)))
       return rc;
     if (q.gated) e = launch_tile<float, true>(a, pairs, stream);
     else if (q.out_type == MM_DTYPE_FP32) e = launch_tile<float, false>(a, pairs, stream);
@@ -819,7 +844,7 @@ int run(const char *what, const Product &q, void *stream) {
   }
   if ((rc = w_map(q.gated ? kRowsM / 2 : kRowsM))) return rc;
   int bn = 16;
-  while (bn < q.tokens) bn *= 2;
+  while (bn < q.tokens && bn < 128) bn *= 2;
   if ((rc = x_map(bn))) return rc;
   switch (q.gated ? -bn : bn) {
     case 16: e = launch_stream<16, false>(a, stream); break;
