@@ -519,24 +519,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
     const int half = e >> 2;                       // this warp's chunks: half, half + 2, ...
     float *ws = scales + e * kScaleFloats, *second = ws + kScaleFloats / 2;  // second: the bias, or the up rows' scales
     const uint32_t mine = out_stage + e * kOutBytes;
+    // a tile's scales: this lane's share, fetched while the tile before it is finished
+    constexpr int PER_LANE = kScaleFloats / 2 / 32;
+    float next_w[PER_LANE], next_s[PER_LANE], next_x = 0.0f;
+    auto fetch = [&](int tile) {
+      int tt, ft;
+      tile_at(p, tile, tt, ft);
+      const int t = tt * kTileM + rank * kRowsM + q * 32 + lane, f0 = ft * tile_f, end = min(p.features, f0 + tile_f);
+      next_x = t < p.tokens ? p.x_scale[t] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < PER_LANE; ++k) {
+        const int i = k * 32 + lane, f = f0 + (2 * (i / CH) + half) * CH + i % CH;  // its place among this warp's chunks
+        next_w[k] = f < end ? p.w_scale[f] : 0.0f;
+        next_s[k] = f >= end ? 0.0f : GATED ? p.w_scale[p.features + f] : p.bias ? p.bias[f] : 0.0f;
+      }
+    };
+    if (pair < tiles) fetch(pair);
     int n = 0;
     for (int tile = pair; tile < tiles; tile += pairs, ++n) {
       const int b = n & 1;
       int tt, ft;
       tile_at(p, tile, tt, ft);
-      const int t0 = tt * kTileM + rank * kRowsM + q * 32, t = t0 + lane;
-      const int f0 = ft * tile_f;
-      const float xs = t < p.tokens ? p.x_scale[t] : 0.0f;
+      const int t0 = tt * kTileM + rank * kRowsM + q * 32, f0 = ft * tile_f;
+      const float xs = next_x;
       __syncwarp();
-      for (int i = lane; i < tile_f / 2 + CH; i += 32) {
-        const int f = f0 + (2 * (i / CH) + half) * CH + i % CH;  // its place among this warp's chunks
-        const bool in = i < kScaleFloats / 2 && f < min(p.features, f0 + tile_f);
-        if (i < kScaleFloats / 2) {
-          ws[i] = in ? p.w_scale[f] : 0.0f;
-          second[i] = !in ? 0.0f : GATED ? p.w_scale[p.features + f] : p.bias ? p.bias[f] : 0.0f;
-        }
+#pragma unroll
+      for (int k = 0; k < PER_LANE; ++k) {
+        ws[k * 32 + lane] = next_w[k];
+        second[k * 32 + lane] = next_s[k];
       }
       __syncwarp();
+      if (tile + pairs < tiles) fetch(tile + pairs);
       if (!warp_agrees(mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc))) break;
       tc_fence_after();
       const uint32_t from = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kTileN;
