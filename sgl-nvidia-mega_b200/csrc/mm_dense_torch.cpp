@@ -27,12 +27,27 @@ namespace {
 using at::ScalarType;
 using at::Tensor;
 
+// A type as Python names it.
+std::string type_name(ScalarType t) {
+  switch (t) {
+    case ScalarType::BFloat16: return "bfloat16";
+    case ScalarType::Half: return "float16";
+    case ScalarType::Float: return "float32";
+    case ScalarType::Double: return "float64";
+    case ScalarType::Char: return "int8";
+    case ScalarType::Byte: return "uint8";
+    case ScalarType::Int: return "int32";
+    case ScalarType::Long: return "int64";
+    default: return c10::toString(t);
+  }
+}
+
 int dtype_code(ScalarType t, const char *name) {
   switch (t) {
     case ScalarType::BFloat16: return MM_DTYPE_BF16;
     case ScalarType::Half: return MM_DTYPE_FP16;
     case ScalarType::Float: return MM_DTYPE_FP32;
-    default: TORCH_CHECK_VALUE(false, name, ": bf16, fp16 or fp32, not ", t);
+    default: TORCH_CHECK_VALUE(false, name, ": bf16, fp16 or fp32, not ", type_name(t));
   }
 }
 
@@ -72,9 +87,9 @@ at::Device cuda(const Tensor &t, const char *name) {
 int64_t row_stride(const Tensor &t, const char *name, at::Device device, ScalarType type, int64_t rows, int64_t cols) {
   TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.dim() == 2 && t.scalar_type() == type && t.device() == device &&
                         (rows < 0 || t.size(0) == rows) && (cols < 0 || t.size(1) == cols),
-                    name, ": expected a ", type, " [", rows < 0 ? std::string("T") : std::to_string(rows), ", ",
+                    name, ": expected a ", type_name(type), " [", rows < 0 ? std::string("T") : std::to_string(rows), ", ",
                     cols < 0 ? std::string("K") : std::to_string(cols), "] tensor on ", device, ", got ", shape(t), " ",
-                    t.scalar_type(), " on ", t.device());
+                    type_name(t.scalar_type()), " on ", t.device());
   TORCH_CHECK_VALUE(t.size(1) <= 1 || t.stride(1) == 1, name, ": rows must be contiguous (stride 1 along the last dimension)");
   TORCH_CHECK_VALUE(t.size(0) < (int64_t(1) << 31) && t.size(1) < (int64_t(1) << 31), name, ": sizes below 2^31, got ", shape(t));
   return t.size(0) > 1 ? t.stride(0) : std::max<int64_t>(t.size(1), 1);
@@ -94,8 +109,8 @@ int64_t code_stride(const Tensor &t, const char *name, at::Device device, int64_
 void *values(const Tensor &t, const char *name, int64_t n, at::Device device, ScalarType type) {
   TORCH_CHECK_VALUE(t.layout() == at::kStrided && t.scalar_type() == type && t.numel() == n && t.dim() >= 1 && t.size(0) == n &&
                         t.device() == device && t.is_contiguous(),
-                    name, ": expected ", n, " contiguous ", type, " values on ", device, ", got ", shape(t), " ",
-                    t.scalar_type(), " on ", t.device());
+                    name, ": expected ", n, " contiguous ", type_name(type), " values on ", device, ", got ", shape(t), " ",
+                    type_name(t.scalar_type()), " on ", t.device());
   return t.data_ptr();
 }
 
@@ -141,8 +156,8 @@ PyObject *rms_norm(PyObject *, PyObject *const *v, Py_ssize_t n) {
   }
   TORCH_CHECK_VALUE(hidden >= 1 && (m.quant != MM_QUANT_MXFP8 || hidden % 32 == 0), "rows of ", hidden,
                     " values (mxfp8: a multiple of 32)");
-  TORCH_CHECK_VALUE(gamma.scalar_type() == type || gamma.scalar_type() == ScalarType::Float, "gamma: ", type, " or fp32, not ",
-                    gamma.scalar_type());
+  TORCH_CHECK_VALUE(gamma.scalar_type() == type || gamma.scalar_type() == ScalarType::Float, "gamma: ", type_name(type), " or fp32, not ",
+                    type_name(gamma.scalar_type()));
   m.gamma_dtype = dtype_code(gamma.scalar_type(), "gamma");
   m.gamma = values(gamma, "gamma", hidden, device, gamma.scalar_type());
   m.eps = static_cast<float>(a.number(2, "eps"));

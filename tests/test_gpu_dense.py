@@ -220,7 +220,9 @@ def test_quantize_extremes():
 
 LINEAR = [(1, 128, 128), (1, 4096, 7168), (1, 1, 1), (2, 7, 16), (5, 129, 130), (16, 300, 1000), (17, 256, 2048), (33, 1000, 512),
           (64, 2311, 5104), (65, 100, 640), (128, 512, 1024), (129, 640, 384), (255, 130, 4096), (256, 384, 256),
-          (257, 384, 256), (300, 1000, 777), (512, 512, 512), (1000, 1100, 1300), (2049, 513, 129), (4096, 2048, 1024)]
+          (257, 384, 256), (300, 1000, 777), (512, 512, 512), (1000, 1100, 1300), (2049, 513, 129), (4096, 2048, 1024),
+          # few features of great depth: the stream form by tiles of 128 tokens
+          (200, 70, 12000), (513, 64, 20000), (1000, 300, 8000), (131, 1, 131071)]
 
 
 @pytest.mark.parametrize("tokens,features,depth", LINEAR)
@@ -305,6 +307,7 @@ def ffn_reference(x, xs, w13, s13, w2, s2, clamp):
 @pytest.mark.parametrize("tokens,hidden,inter,clamp", [
     (1, 7168, 2048, None), (1, 128, 64, 2.0), (3, 250, 130, None), (8, 1024, 512, 1.0), (16, 512, 1990, None), (40, 640, 300, 2.5),
     (80, 512, 1000, None), (128, 384, 256, 2.0), (200, 520, 264, None), (257, 256, 384, 1.5), (600, 1000, 700, None), (1024, 2048, 1024, None),
+    (200, 6000, 100, 1.0), (200, 256, 16000, None),  # one product in either form
 ])
 @pytest.mark.parametrize("dtype", [BF, FH, F32])
 def test_ffn(tokens, hidden, inter, clamp, dtype):
@@ -377,6 +380,19 @@ def test_weights_written_just_before_the_call():
         got.append(megamoe.int8_ffn(x, xs, w13, s13, w2, s2))
     for k, y in enumerate(got):
         assert torch.equal(y, want[k % 2]), k
+    # a gated product of many tokens before a down product that loads early
+    x, xs = weights(200, 256, g)
+    w13, s13 = weights(2 * 8192, 256, g)
+    w2a, s2 = weights(256, 8192, g)
+    w2b = w2a.flip(0).contiguous()
+    want = [megamoe.int8_ffn(x, xs, w13, s13, b, s2) for b in (w2a, w2b)]
+    w2 = w2a.clone()
+    for k in range(20):
+        w2.copy_(w2b if k % 2 else w2a)
+        y = megamoe.int8_ffn(x, xs, w13, s13, w2, s2)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[k % 2]), k
+    x, xs = weights(4, 1024, g)
     # and by an operator of this library that lets its successor start early
     f = randn((4096, 1024), g)
     for k in range(20):
@@ -436,6 +452,12 @@ def test_refusals():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"call {i} was not refused")
+
+
+def test_refusals_name_types_as_torch_does():
+    q, s = torch.zeros((4, 64), dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")
+    with pytest.raises(ValueError, match=r"weight: expected a int8 \[T, 64\] tensor on cuda:0, got \[4, 64\] float32 on cuda:0"):
+        megamoe.int8_linear(q, s, q.float(), s)
 
 
 def test_streams_and_graphs():
