@@ -317,7 +317,9 @@ int mm_finalize_partial(const float *partial, uint16_t *out, int32_t tokens,
  *   norm_out = round(y); codes and scales of y (not of the rounded norm)
  * What the reference's hop fuses behind its all-reduce (deepseek_v41/sm103/
  * all_reduce_mhc.py:665-1190: RMSNorm and the MXFP8 of the next input), for one
- * GPU's rows. Like every call below: on the current device, which holds the
+ * GPU's rows. residual_out may be x or residual (same row stride); apart from that
+ * no output shares memory with an input or another output. At most 2^30 tokens and
+ * values a row. Like every call below: on the current device, which holds the
  * buffers; 0 tokens launch nothing. */
 int mm_rms_norm(const mm_norm_args *args, void *stream);
 
@@ -328,7 +330,7 @@ int mm_quantize_int8(const void *x, int64_t ld_x, int32_t dtype, int8_t *codes, 
 /* out[t, n] = round((sum_k x[t, k] w[n, k]) * x_scale[t] * w_scale[n] + bias[n]):
  * int8 codes with a scale per token and per channel, the sum an exact 32-bit integer.
  * x and w rows start on 16-byte boundaries (base and row stride); bias fp32 or NULL.
- * depth < 131072. */
+ * depth < 131072, tokens < 2^23, features at most 2^30; out shares no memory with an input. */
 int mm_int8_linear(const int8_t *x, int64_t ld_x, const float *x_scale, const int8_t *w, int64_t ld_w,
                    const float *w_scale, const float *bias, void *out, int64_t ld_out,
                    int32_t out_dtype, int32_t tokens, int32_t features, int32_t depth, void *stream);

@@ -769,6 +769,8 @@ int run_norm(const char *what, NormArgs a, int dtype, int quant, void *stream) {
     return set_error(MM_ERR_INVALID, "%s: unknown type %d", what, dtype);
   if (quant != MM_QUANT_NONE && quant != MM_QUANT_MXFP8 && quant != MM_QUANT_INT8)
     return set_error(MM_ERR_INVALID, "%s: unknown 8-bit format %d", what, quant);
+  if (a.tokens > 1 << 30 || a.hidden > 1 << 30)
+    return set_error(MM_ERR_UNSUPPORTED, "%s: %d tokens of %d values: at most 2^30 of each", what, a.tokens, a.hidden);
   if (a.tokens == 0) return MM_OK;
   if (!a.x || (quant && (!a.codes || !a.scales)) || (!quant && !a.norm_out))
     return set_error(MM_ERR_INVALID, "%s: null pointer", what);
@@ -782,15 +784,27 @@ int run_norm(const char *what, NormArgs a, int dtype, int quant, void *stream) {
     return set_error(MM_ERR_INVALID, "%s: rows overlap (a row stride below %d)", what, a.hidden);
   const int es = dtype_bytes(dtype);
   // each thread writes the residual over elements that it alone has read, so that it may take
-  // x's or the residual's own place, row for row; no other buffers may overlap
-  auto bytes = [&](int64_t ld) { return ((a.tokens - 1) * ld + a.hidden) * es; };
-  auto clash = [&](const void *p, int64_t ld_p, const void *q, int64_t ld_q) { return overlap(p, bytes(ld_p), q, bytes(ld_q)); };
-  auto moved = [&](const void *in, int64_t ld) {
-    return clash(in, ld, a.residual_out, a.ld_residual_out) && !(in == a.residual_out && ld == a.ld_residual_out);
+  // x's or the residual's own place, row for row; no other buffers may share memory with an output
+  struct Buffer {
+    const void *p;
+    int64_t bytes;
   };
-  if (clash(a.x, a.ld_x, a.norm_out, a.ld_norm) || clash(a.residual, a.ld_residual, a.norm_out, a.ld_norm) ||
-      clash(a.residual_out, a.ld_residual_out, a.norm_out, a.ld_norm) || moved(a.x, a.ld_x) || moved(a.residual, a.ld_residual))
-    return set_error(MM_ERR_INVALID, "%s: an output overlaps another buffer", what);
+  auto rows = [&](const void *p, int64_t ld, int size) { return Buffer{p, ((a.tokens - 1) * ld + a.hidden) * size}; };
+  const Buffer in[] = {rows(a.x, a.ld_x, es), rows(a.residual, a.ld_residual, es),
+                       {a.gamma, static_cast<int64_t>(a.hidden) * (a.gamma_f32 ? 4 : es)}};
+  const int64_t scale_bytes = quant == MM_QUANT_MXFP8 ? static_cast<int64_t>(a.tokens) * (a.hidden / 32) : static_cast<int64_t>(a.tokens) * 4;
+  const Buffer out[] = {rows(a.residual_out, a.ld_residual_out, es), rows(a.norm_out, a.ld_norm, es),
+                        rows(quant ? a.codes : nullptr, a.ld_codes, 1), {quant ? a.scales : nullptr, scale_bytes}};
+  auto in_place = [&](const Buffer &o, const Buffer &i) {
+    return &o == out && o.p == i.p && ((&i == in && a.ld_x == a.ld_residual_out) || (&i == in + 1 && a.ld_residual == a.ld_residual_out));
+  };
+  for (const Buffer &o : out) {
+    for (const Buffer &i : in)
+      if (overlap(o.p, o.bytes, i.p, i.bytes) && !in_place(o, i))
+        return set_error(MM_ERR_INVALID, "%s: an output overlaps an input", what);
+    for (const Buffer &other : out)
+      if (&other < &o && overlap(o.p, o.bytes, other.p, other.bytes)) return set_error(MM_ERR_INVALID, "%s: an output overlaps another", what);
+  }
   const uintptr_t base = reinterpret_cast<uintptr_t>(a.x);
   bool wide = true;
   auto same = [&](const void *p, int64_t ld) {

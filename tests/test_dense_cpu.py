@@ -62,6 +62,28 @@ def test_norm_refusals(bad, word):
     assert word in L.mm_last_error(), L.mm_last_error()
 
 
+@pytest.mark.parametrize("bad", [
+    dict(norm_out=BASE + 4096 - 64), dict(codes=BASE + 64), dict(codes=BASE + 4096), dict(scales=BASE + 12288 + 32),
+    dict(codes=BASE + 20480), dict(residual_out=BASE + 4096), dict(scales=BASE + 8192),
+    dict(codes=BASE + 24576 + 192), dict(gamma=BASE + 12288 - 124, gamma_dtype=_lib.MM_DTYPE_FP32),
+])
+def test_norm_outputs_share_no_memory(bad):
+    L = _lib.lib()
+    assert L.mm_rms_norm(ctypes.byref(norm_args(**bad)), None) == _lib.MM_ERR_INVALID
+    assert b"overlaps" in L.mm_last_error(), L.mm_last_error()
+
+
+MOST = 1 << 30
+
+
+@pytest.mark.parametrize("tokens,hidden", [(1, MOST + 1), (2 ** 31 - 1, 1), (1, 2 ** 31 - 1), (0, MOST + 1)])
+def test_row_kernels_sizes(tokens, hidden):
+    L = _lib.lib()
+    big = dict(tokens=tokens, hidden=hidden, **{f: hidden for f in ("ld_x", "ld_residual", "ld_residual_out", "ld_norm", "ld_codes")})
+    assert L.mm_rms_norm(ctypes.byref(norm_args(**big)), None) == _lib.MM_ERR_UNSUPPORTED
+    assert L.mm_quantize_int8(BASE, hidden, 0, BASE, hidden, BASE, tokens, hidden, None) == _lib.MM_ERR_UNSUPPORTED
+
+
 def test_empty_calls_launch_nothing():
     L = _lib.lib()
     assert L.mm_rms_norm(ctypes.byref(norm_args(tokens=0)), None) == _lib.MM_OK
@@ -91,6 +113,28 @@ def linear(**kw):
 def test_linear_refusals(bad, status):
     assert linear(**bad) == status
     assert b"mm_int8_linear" in _lib.lib().mm_last_error()
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(out=BASE + 40960, xs=BASE + 40960 + 124), 1), (dict(out=BASE + 40960, ws=BASE + 40960 - 124), 1),
+    (dict(out=BASE + 40960, bias=BASE + 40960), 1), (dict(features=MOST + 1, ld_out=MOST + 1), 2),
+])
+def test_linear_output_and_sizes(bad, status):
+    assert linear(**bad) == status
+
+
+@pytest.mark.parametrize("name,at", [("x", 0), ("w13", 256), ("w2", 256), ("x_scale", 300), ("w13_scale", 300), ("w2_scale", 300), ("out", 256)])
+def test_ffn_workspace_overlaps(name, at):
+    L = _lib.lib()
+    assert L.mm_int8_ffn(ctypes.byref(ffn_args(**{name: BASE + 4096 * 7 + at})), None) == _lib.MM_ERR_INVALID
+    assert b"overlaps" in L.mm_last_error(), L.mm_last_error()
+
+
+@pytest.mark.parametrize("name", ["x", "x_scale", "w13", "w13_scale", "w2", "w2_scale"])
+def test_ffn_output_overlaps(name):
+    L = _lib.lib()
+    assert L.mm_int8_ffn(ctypes.byref(ffn_args(**{name: BASE + 4096 * 6})), None) == _lib.MM_ERR_INVALID
+    assert b"overlaps an input" in L.mm_last_error(), L.mm_last_error()
 
 
 def ffn_args(**kw):
