@@ -125,15 +125,18 @@ struct Stream {
   // 4096 x 7168 7.3 and 7.7, 16 x 7168 x 7168 10.6 and 11.0, 64 x 7168 x 7168 12.9 and 12.4, 128 x
   // 7168 x 7168 16.5 and 15.0): a send moves 4 bytes a lane, a read 16.
   static constexpr bool kPush = BN <= 32;
+  // Warp 0 loads, warp 1 issues the products, kGroups of four warps read the sums, all of them add
+  // the parts. More warps start later and finish more tokens at once (us with 6, 8 and 10: 1 x 7168
+  // x 2048 4.6, 4.8, 4.9; 64 x 2048 x 7168 7.95, 7.6, 7.6; 80 x 2048 x 7168 8.8, 9.1, 8.7; 128 x 18432 x 7168
+  // 26.9, 26.0, 25.8).
+  static constexpr int kWarps = BN <= 32 ? 6 : BN == 64 ? 8 : 10;
+  static constexpr int kGroups = (kWarps - 2) / 4;
   static_assert(kStages >= 2 && kCols <= 256, "two CTAs an SM share 512 columns");
   static_assert(BN * kRowsM * 4 <= kStages * kStageBytes, "the parts take the ring's place");
 };
 
-constexpr int kStreamThreads = 192;
-constexpr int kStreamWarps = kStreamThreads / 32;
-
 template <int BN, bool GATED>
-__global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __grid_constant__ Int8Args p) {
+__global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_kernel(const __grid_constant__ Int8Args p) {
   using S = Stream<BN, GATED>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -263,9 +266,9 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   bool ok = mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc);
   tc_fence_after();
   ok = ok && *failed == 0u;
-  // Every CTA of the cluster finishes the tokens rank, rank + split, ... Warps 2..5 read the sums
-  // (warp w: TMEM lanes 32 (w % 4) and on, weight rows; a column a token).
-  const int q = warp & 3;
+  // Every CTA of the cluster finishes the tokens rank, rank + split, ... Groups of four warps read the
+  // sums (warp w: TMEM lanes 32 (w % 4) and on, weight rows; a column a token), 16 tokens in turn.
+  const int q = warp & 3, group = warp < 2 ? -1 : (warp - 2) >> 2;
   const uint32_t sums = tmem + (static_cast<uint32_t>(q * 32) << 16);
   auto finish = [&](int j, int4 sum) {
     const float xs = x_scale[j];
@@ -285,15 +288,15 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     // The parts go into the ring of the CTA that finishes their token, once every CTA of the
     // cluster is past its products: [token's turn][part][weight row].
     cluster_arrive();
-    if (warp >= 2) {
+    if (group >= 0 && group < S::kGroups) {
       const int turns = __ffs(split) - 1;  // split is a power of two
       const uint32_t at = ring + (rank * kRowsM + q * 32 + lane) * 4;
 #pragma unroll 1
-      for (int j = 0; j < live; j += 16) {
+      for (int j = 16 * group; j < live; j += 16 * S::kGroups) {
         uint32_t r[16];
         tc_ld_32x32b_x16(sums + j, r);
         tc_wait_ld();
-        if (j == 0) cluster_wait();
+        if (j == 16 * group) cluster_wait();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int owner = (j + i) & (split - 1), turn = (j + i) >> turns;
@@ -312,7 +315,7 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
       return;
     }
 #pragma unroll 1
-    for (int j = rank + split * warp; j < live; j += split * kStreamWarps) {
+    for (int j = rank + split * warp; j < live; j += split * S::kWarps) {
       const int *part = reinterpret_cast<const int *>(ring_ptr) + (j & ~(split - 1)) * kRowsM + PER * lane;
       int4 sum = make_int4(0, 0, 0, 0);
 #pragma unroll 8
@@ -328,10 +331,11 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
     }
     return;
   }
-  // Each CTA leaves its parts in its own ring, [token][weight row], and reads the others' there.
-  if (warp >= 2) {
+  // Each CTA leaves its parts in its own ring, [token][weight row], and reads the others' there, from
+  // its neighbour on (all from the first CTA's at once: 48 x 2048 x 7168 7.45 us instead of 7.1).
+  if (group >= 0 && group < S::kGroups) {
 #pragma unroll 1
-    for (int j = 0; j < live; j += 16) {
+    for (int j = 16 * group; j < live; j += 16 * S::kGroups) {
       uint32_t r[16];
       tc_ld_32x32b_x16(sums + j, r);
       tc_wait_ld();
@@ -344,12 +348,12 @@ __global__ void __launch_bounds__(kStreamThreads) int8_stream_kernel(const __gri
   cluster_sync();
   if (warp == 1) tmem_dealloc(tmem, S::kCols);
 #pragma unroll 1
-  for (int j = rank + split * warp; j < live; j += split * kStreamWarps) {
+  for (int j = rank + split * warp; j < live; j += split * S::kWarps) {
     const uint32_t at = ring + (j * kRowsM + PER * lane) * 4;
     int4 sum = make_int4(0, 0, 0, 0);
-#pragma unroll 4
+#pragma unroll 2
     for (int r = 0; r < split; ++r) {
-      const uint32_t from = cluster_map(at, r);
+      const uint32_t from = cluster_map(at, (rank + r) & (split - 1));
       if constexpr (GATED) {
         const int2 g = cluster_load_v2(from), u = cluster_load_v2(from + 4 * S::kFeatures);
         add(sum, make_int4(g.x, g.y, u.x, u.y));
@@ -719,7 +723,7 @@ cudaError_t launch_stream(Int8Args &a, void *stream) {
   if (e != cudaSuccess) return e;
   const int tiles = (a.features + S::kFeatures - 1) / S::kFeatures, token_tiles = (a.tokens + BN - 1) / BN;
   a.split = stream_split(tiles * token_tiles, a.blocks_k);
-  return launch_cluster(int8_stream_kernel<BN, GATED>, dim3(tiles * a.split, token_tiles), kStreamThreads, S::kSmem, a.split, stream, a);
+  return launch_cluster(int8_stream_kernel<BN, GATED>, dim3(tiles * a.split, token_tiles), S::kWarps * 32, S::kSmem, a.split, stream, a);
 }
 
 // CTA pairs that the current device runs at once (of the tile form: one CTA an SM, all its
