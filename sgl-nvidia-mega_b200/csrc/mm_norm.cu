@@ -704,10 +704,22 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
 }
 
 // Chunks a thread. Few rows: as few as its threads allow (one row's latency). Many rows: more,
-// so that more loads of more rows are in flight; measured (bf16, us): norm + MXFP8 of 8192 x
-// 7168: two 98, four 83 (6.4 TB/s), eight 101; of 4096 x 16384: four 94, eight 128; of 8192 x
-// 2048: one 28, two 26; of 1024 x 5120: two 8.3, four 10.5, eight 16.8. int8 rows alone hold
-// less beside the row: 4096 x 16384: four 42, eight 35; 8192 x 7168: two 41, four 33, eight 30.5.
+// so that more loads of more rows are in flight and fewer warps meet at a barrier; measured (bf16,
+// us): norm + MXFP8 of 8192 x 7168: two 103, four 83 (6.4 TB/s), eight 101; of 1024 x 7168: two 14.4,
+// four 12.7; of 4096 x 16384: four 94, eight 128; of 8192 x 2048: two 25.6, four 26.0. Rows between:
+// what takes fewer rounds of the GPU (norm of 520 x 6147: two 7.0, four 5.2; of 640 x 6147: two 7.3,
+// four 8.3; of 1024 x 5120: two 6.2, four 7.3); fp32 rows without int8 fit more often and stay at two
+// (1021 x 3001: two 6.7, four 7.5). int8 rows alone hold less beside the row: 4096 x 16384: four 42, eight
+// 35; 8192 x 7168: two 41, four 33, eight 30.5.
+// Rows that the GPU's SMs hold at once with nv (two or four) chunks a thread, 48 or 64 registers.
+int rows_at_once(int nv, int chunks) {
+  const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
+  return 148 * std::min(65536 / (threads * (nv == 2 ? 48 : 64)), 2048 / threads);
+}
+bool fewer_rounds(int tokens, int chunks) {
+  auto rounds = [&](int nv) { return (tokens + rows_at_once(nv, chunks) - 1) / rows_at_once(nv, chunks); };
+  return rounds(4) < rounds(2);
+}
 template <typename T, int QUANT, bool NORM, bool TURN>
 cudaError_t launch_rows(NormArgs a, int chunks, void *stream) {
   a.turn_bytes = TURN ? static_cast<int>((chunks * (16 / sizeof(T)) + 32) / 16 * 16 + 16) : 0;
@@ -718,7 +730,8 @@ cudaError_t launch_rows(NormArgs a, int chunks, void *stream) {
   if (share > 1) nv = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
   else if (a.tokens <= kFewRows) nv = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
   else if (!NORM) nv = chunks <= 256 ? 2 : chunks <= 512 ? 4 : 8;
-  else nv = chunks <= (a.tokens <= 2048 ? 1024 : 512) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
+  else if (sizeof(T) == 4 && QUANT != MM_QUANT_INT8) nv = chunks <= (a.tokens <= 2048 ? 1024 : 512) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
+  else nv = chunks <= 512 || (chunks <= 832 && a.tokens <= 2048 && !fewer_rounds(a.tokens, chunks)) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
   auto go = [&](auto kernel, int n) {
     const dim3 block = share > 1 ? dim3(32, share) : dim3(((chunks + n - 1) / n + 31) / 32 * 32);
     return launch(kernel, dim3((a.tokens + share - 1) / share), block, share * a.turn_bytes, stream, a);
