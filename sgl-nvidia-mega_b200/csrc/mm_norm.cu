@@ -319,10 +319,12 @@ __device__ __forceinline__ uint4 gamma_chunk(const NormArgs &a, int e0) {
 // the 64 registers that 1024 threads leave each.
 // CTAs that shall share an SM: two of fp32 rows (h of a wide layer, 4096 x 18432: 70 us instead
 // of 92; 16-bit rows lose by it, 8192 x 7168 36 instead of 30), one of the latency form.
-constexpr int row_ctas(int nv, bool norm, int es) { return nv == 8 && !norm && es == 4 ? 2 : nv == 1 ? 1 : 0; }
-constexpr int row_threads(int nv, bool norm) { return nv >= 8 && norm ? 512 : nv >= 4 ? 640 : 1024; }
-template <typename T, int NV, int QUANT, bool NORM, bool TURN>
-__global__ void __launch_bounds__(row_threads(NV, NORM), row_ctas(NV, NORM, sizeof(T))) norm_rows_kernel(const __grid_constant__ NormArgs a) {
+// DENSE: 56 registers instead of 64 and five CTAs of 224 threads instead of four (norm alone of 8192 x
+// 7168 48.0 us, so 42.7; of 8192 x 6147 56.2 and 49.7; beside codes it spills).
+constexpr int row_ctas(int nv, bool norm, int es, bool dense) { return dense ? 4 : nv == 8 && !norm && es == 4 ? 2 : nv == 1 ? 1 : 0; }
+constexpr int row_threads(int nv, bool norm, bool dense = false) { return dense ? 288 : nv >= 8 && norm ? 512 : nv >= 4 ? 640 : 1024; }
+template <typename T, int NV, int QUANT, bool NORM, bool TURN, bool DENSE>
+__global__ void __launch_bounds__(row_threads(NV, NORM, DENSE), row_ctas(NV, NORM, sizeof(T), DENSE)) norm_rows_kernel(const __grid_constant__ NormArgs a) {
   using C = Chunk<T>;
   constexpr int VEC = C::kVec, PAIRS = C::kPairs;
   __shared__ double red_d[32];
@@ -711,14 +713,14 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
 // four 8.3; of 1024 x 5120: two 6.2, four 7.3); fp32 rows without int8 fit more often and stay at two
 // (1021 x 3001: two 6.7, four 7.5). int8 rows alone hold less beside the row: 4096 x 16384: four 42, eight
 // 35; 8192 x 7168: two 41, four 33, eight 30.5.
-// Rows that the GPU's SMs hold at once with nv (two or four) chunks a thread, 48 or 64 registers.
-int rows_at_once(int nv, int chunks) {
-  const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32;
-  return 148 * std::min(65536 / (threads * (nv == 2 ? 48 : 64)), 2048 / threads);
-}
-bool fewer_rounds(int tokens, int chunks) {
-  auto rounds = [&](int nv) { return (tokens + rows_at_once(nv, chunks) - 1) / rows_at_once(nv, chunks); };
-  return rounds(4) < rounds(2);
+// Whether four chunks a thread (of `regs` registers) take fewer rounds than two (of 48): the rows
+// that the SMs hold at once decide.
+bool fewer_rounds(int tokens, int chunks, int regs) {
+  auto rounds = [&](int nv, int r) {
+    const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32, rows = 148 * std::min(65536 / (threads * r), 2048 / threads);
+    return (tokens + rows - 1) / rows;
+  };
+  return rounds(4, regs) < rounds(2, 48);
 }
 template <typename T, int QUANT, bool NORM, bool TURN>
 cudaError_t launch_rows(NormArgs a, int chunks, void *stream) {
@@ -731,16 +733,18 @@ cudaError_t launch_rows(NormArgs a, int chunks, void *stream) {
   else if (a.tokens <= kFewRows) nv = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
   else if (!NORM) nv = chunks <= 256 ? 2 : chunks <= 512 ? 4 : 8;
   else if (sizeof(T) == 4 && QUANT != MM_QUANT_INT8) nv = chunks <= (a.tokens <= 2048 ? 1024 : 512) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
-  else nv = chunks <= 512 || (chunks <= 832 && a.tokens <= 2048 && !fewer_rounds(a.tokens, chunks)) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
+  else nv = chunks <= 512 || (chunks <= 832 && a.tokens <= 2048 && !fewer_rounds(a.tokens, chunks, QUANT == MM_QUANT_NONE ? 56 : 64)) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
   auto go = [&](auto kernel, int n) {
     const dim3 block = share > 1 ? dim3(32, share) : dim3(((chunks + n - 1) / n + 31) / 32 * 32);
     return launch(kernel, dim3((a.tokens + share - 1) / share), block, share * a.turn_bytes, stream, a);
   };
+  if constexpr (QUANT == MM_QUANT_NONE && sizeof(T) == 2)
+    if (nv == 4 && share == 1 && chunks <= 4 * row_threads(4, NORM, true)) return go(norm_rows_kernel<T, 4, QUANT, NORM, TURN, true>, 4);
   switch (nv) {
-    case 1: return go(norm_rows_kernel<T, 1, QUANT, NORM, TURN>, 1);
-    case 2: return go(norm_rows_kernel<T, 2, QUANT, NORM, TURN>, 2);
-    case 4: return go(norm_rows_kernel<T, 4, QUANT, NORM, TURN>, 4);
-    default: return go(norm_rows_kernel<T, 8, QUANT, NORM, TURN>, 8);
+    case 1: return go(norm_rows_kernel<T, 1, QUANT, NORM, TURN, false>, 1);
+    case 2: return go(norm_rows_kernel<T, 2, QUANT, NORM, TURN, false>, 2);
+    case 4: return go(norm_rows_kernel<T, 4, QUANT, NORM, TURN, false>, 4);
+    default: return go(norm_rows_kernel<T, 8, QUANT, NORM, TURN, false>, 8);
   }
 }
 
