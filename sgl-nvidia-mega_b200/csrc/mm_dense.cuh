@@ -6,9 +6,6 @@
 
 namespace mm {
 
-// Up to this many rows a row kernel spreads each over as many threads as it has 16-byte
-// chunks; beyond, rows share the SMs.
-constexpr int kFewRows = 296;
 // Short rows share CTAs from this many on (four CTAs an SM at four rows each).
 constexpr int kShareRows = 4 * 592;
 

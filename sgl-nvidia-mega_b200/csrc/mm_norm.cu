@@ -705,47 +705,62 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
   }
 }
 
-// Chunks a thread. Few rows: as few as its threads allow (one row's latency). Many rows: more,
-// so that more loads of more rows are in flight and fewer warps meet at a barrier; measured (bf16,
-// us): norm + MXFP8 of 8192 x 7168: two 103, four 83 (6.4 TB/s), eight 101; of 1024 x 7168: two 14.4,
-// four 12.7; of 4096 x 16384: four 94, eight 128; of 8192 x 2048: two 25.6, four 26.0. Rows between:
-// what takes fewer rounds of the GPU (norm of 520 x 6147: two 7.0, four 5.2; of 640 x 6147: two 7.3,
-// four 8.3; of 1024 x 5120: two 6.2, four 7.3); fp32 rows without int8 fit more often and stay at two
-// (1021 x 3001: two 6.7, four 7.5). int8 rows alone hold less beside the row: 4096 x 16384: four 42, eight
-// 35; 8192 x 7168: two 41, four 33, eight 30.5.
-// Whether four chunks a thread (of `regs` registers) take fewer rounds than two (of 48): the rows
-// that the SMs hold at once decide.
-bool fewer_rounds(int tokens, int chunks, int regs) {
-  auto rounds = [&](int nv, int r) {
-    const int threads = ((chunks + nv - 1) / nv + 31) / 32 * 32, rows = 148 * std::min(65536 / (threads * r), 2048 / threads);
-    return (tokens + rows - 1) / rows;
-  };
-  return rounds(4, regs) < rounds(2, 48);
+// The registers of a thread of a kernel, as it was compiled.
+template <auto KERNEL>
+int registers() {
+  static const int regs = [] {
+    cudaFuncAttributes f = {};
+    return cudaFuncGetAttributes(&f, KERNEL) == cudaSuccess ? (f.numRegs + 7) / 8 * 8 : 64;
+  }();
+  return regs;
 }
+// Rounds that the GPU's 148 SMs need for `tokens` rows of `warps` warps each.
+int rounds(int tokens, int warps, int regs) {
+  const int rows = 148 * std::max(1, std::min(4 * (512 / regs), 64) / warps);
+  return (tokens + rows - 1) / rows;
+}
+
+// Chunks a thread. As few as hold all rows in the SMs at once (one row's latency; norm + MXFP8 + residual
+// of 256 x 7168: one chunk, two rounds 6.4 us, two chunks, one round 4.6). More rows than that:
+// more chunks, so that more loads of more rows are in flight and fewer warps meet at a barrier (bf16,
+// us: norm + MXFP8 of 8192 x 7168: two 103, four 83 (6.4 TB/s), eight 101; of 4096 x 16384: four 94, eight 128;
+// of 8192 x 2048: two 25.6, four 26.0), rows between by the rounds (norm of 640 x 6147: two 7.3, four
+// 8.3; of 1024 x 6147: two 9.9, four 9.0). int8 rows alone hold less beside the row: 4096 x 16384: four
+// 42, eight 35; 8192 x 7168: two 41, four 33, eight 30.5.
 template <typename T, int QUANT, bool NORM, bool TURN>
 cudaError_t launch_rows(NormArgs a, int chunks, void *stream) {
+  constexpr bool kDense = QUANT == MM_QUANT_NONE && sizeof(T) == 2;
+  constexpr auto one = norm_rows_kernel<T, 1, QUANT, NORM, TURN, false>;
+  constexpr auto two = norm_rows_kernel<T, 2, QUANT, NORM, TURN, false>;
+  constexpr auto four = norm_rows_kernel<T, 4, QUANT, NORM, TURN, false>;
+  constexpr auto eight = norm_rows_kernel<T, 8, QUANT, NORM, TURN, false>;
   a.turn_bytes = TURN ? static_cast<int>((chunks * (16 / sizeof(T)) + 32) / 16 * 16 + 16) : 0;
   // Short rows in number share CTAs, a warp each (int8 rows of 8192 x 1024 5.4 us instead of 9.2,
   // norm of 8192 x 512 6.1 instead of 9.4; norm with int8 of 1300 x 1024 6.0 instead of 4.4).
   const int share = chunks > 128 || a.tokens < kShareRows ? 1 : a.tokens < 2 * kShareRows ? 4 : 8;
+  const bool dense = kDense && share == 1 && chunks <= 4 * row_threads(4, NORM, true);
+  auto warps = [&](int n) { return (chunks + 32 * n - 1) / (32 * n); };
+  auto in_one_round = [&](int n, int regs) { return chunks <= n * row_threads(n, NORM) && rounds(a.tokens, warps(n), regs) == 1; };
   int nv;
+  int regs4 = registers<four>();
+  if constexpr (kDense)
+    if (dense) regs4 = registers<norm_rows_kernel<T, 4, QUANT, NORM, TURN, true>>();
   if (share > 1) nv = chunks <= 32 ? 1 : chunks <= 64 ? 2 : 4;
-  else if (a.tokens <= kFewRows) nv = chunks <= 1024 ? 1 : chunks <= 2048 ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
+  else if (in_one_round(1, registers<one>())) nv = 1;
+  else if (in_one_round(2, registers<two>())) nv = 2;
+  else if (chunks > 4 * row_threads(4, NORM)) nv = 8;
+  else if ((chunks > 512 || QUANT == MM_QUANT_NONE) && in_one_round(4, regs4)) nv = 4;
   else if (!NORM) nv = chunks <= 256 ? 2 : chunks <= 512 ? 4 : 8;
-  else if (sizeof(T) == 4 && QUANT != MM_QUANT_INT8) nv = chunks <= (a.tokens <= 2048 ? 1024 : 512) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
-  else nv = chunks <= 512 || (chunks <= 832 && a.tokens <= 2048 && !fewer_rounds(a.tokens, chunks, QUANT == MM_QUANT_NONE ? 56 : 64)) ? 2 : chunks <= 4 * row_threads(4, NORM) ? 4 : 8;
+  else if (chunks <= 512) nv = 2;
+  else if (chunks <= 832 && a.tokens <= 2048) nv = rounds(a.tokens, warps(4), regs4) < rounds(a.tokens, warps(2), registers<two>()) ? 4 : 2;
+  else nv = 4;
   auto go = [&](auto kernel, int n) {
     const dim3 block = share > 1 ? dim3(32, share) : dim3(((chunks + n - 1) / n + 31) / 32 * 32);
     return launch(kernel, dim3((a.tokens + share - 1) / share), block, share * a.turn_bytes, stream, a);
   };
-  if constexpr (QUANT == MM_QUANT_NONE && sizeof(T) == 2)
-    if (nv == 4 && share == 1 && chunks <= 4 * row_threads(4, NORM, true)) return go(norm_rows_kernel<T, 4, QUANT, NORM, TURN, true>, 4);
-  switch (nv) {
-    case 1: return go(norm_rows_kernel<T, 1, QUANT, NORM, TURN, false>, 1);
-    case 2: return go(norm_rows_kernel<T, 2, QUANT, NORM, TURN, false>, 2);
-    case 4: return go(norm_rows_kernel<T, 4, QUANT, NORM, TURN, false>, 4);
-    default: return go(norm_rows_kernel<T, 8, QUANT, NORM, TURN, false>, 8);
-  }
+  if constexpr (kDense)
+    if (nv == 4 && dense) return go(norm_rows_kernel<T, 4, QUANT, NORM, TURN, true>, 4);
+  return nv == 1 ? go(one, 1) : nv == 2 ? go(two, 2) : nv == 4 ? go(four, 4) : go(eight, 8);
 }
 
 template <typename T, int QUANT>
