@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from ._lib import check, lib
-from .moe import _ptr, _stream
+from .moe import _ptr, _stream, check_shared_output
 
 
 class PeerAllReduce:
@@ -106,11 +106,10 @@ class PeerAllReduce:
             raise ValueError(f"rows must be bf16 [rows, {self.hidden}]")
         if weights.dtype != torch.float32 or permuted.dtype != torch.int32 or tuple(permuted.shape) != (tokens, top_k):
             raise ValueError("weights fp32 [T, k] and permuted int32 [T, k] expected")
-        if shared_output is not None and (shared_output.dtype != torch.bfloat16
-                                          or tuple(shared_output.shape) != (tokens, self.hidden)):
-            raise ValueError("shared_output must be bf16 [T, H]")
-        for t in (rows, weights, permuted, shared_output):
-            if t is not None and not t.is_contiguous():
+        if shared_output is not None:
+            check_shared_output(shared_output, tokens, self.hidden, rows.device)
+        for t in (rows, weights, permuted):
+            if not t.is_contiguous():
                 raise ValueError("finalize inputs must be contiguous")
         return tokens, top_k
 

@@ -52,6 +52,13 @@ def _expect(t: torch.Tensor, shape: Sequence[int], name: str, nbytes: int = 1) -
     return t
 
 
+def check_shared_output(t: torch.Tensor, tokens: int, hidden: int, device: torch.device) -> None:
+    """Refuse rows that the combine, which reads bf16 [T, H] end to end, cannot add."""
+    if t.dtype != torch.bfloat16 or tuple(t.shape) != (tokens, hidden) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"shared_output must be contiguous bf16 [{tokens}, {hidden}] on {device}, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
+
+
 def _u8(t: torch.Tensor) -> torch.Tensor:
     return t.view(torch.uint8) if t.element_size() == 1 and t.dtype != torch.uint8 else t
 
@@ -380,9 +387,7 @@ class RoutedMoE:
         if shared_output is not None:
             if self.has_shared:
                 raise ValueError("forward: shared_output needs a layer without a shared expert of its own")
-            if shared_output.dtype != torch.bfloat16 or tuple(shared_output.shape) != (tokens, self.hidden) \
-                    or not shared_output.is_contiguous() or shared_output.device != self.device:
-                raise ValueError(f"shared_output must be contiguous bf16 [T, {self.hidden}] on {self.device}")
+            check_shared_output(shared_output, tokens, self.hidden, self.device)
         b = {} if buffers is None else buffers
         dev = self.device
         if router_weight is not None:
@@ -591,10 +596,14 @@ def route(ids: torch.Tensor, experts: int, expert_offset: int = 0):
 
 def finalize(rows: torch.Tensor, weights: torch.Tensor, permuted: torch.Tensor,
              shared_output: Optional[torch.Tensor] = None, partial: bool = False) -> torch.Tensor:
-    """out[t] = bf16(bf16(sum_k w * rows[perm]) + shared[t]) in slot order."""
+    """out[t] = bf16(bf16(sum_k w * rows[perm]) + shared[t]) in slot order.
+    ``shared_output``: contiguous bf16 [T, H] beside ``rows`` (of a longer one
+    the first T rows)."""
     tokens, top_k = permuted.shape
     hidden = rows.size(1)
     dev = rows.device
+    if shared_output is not None:
+        check_shared_output(shared_output[:tokens], tokens, hidden, dev)
     out = None if partial else torch.empty((tokens, hidden), dtype=torch.bfloat16, device=dev)
     part = torch.empty((2, tokens, hidden), dtype=torch.float32, device=dev) if partial else None
     w = weights.to(torch.float32).contiguous()
