@@ -98,7 +98,7 @@ int64_t row_stride(const Tensor &t, const char *name, at::Device device, ScalarT
 // The same of int8 rows, which start on 16-byte boundaries.
 int64_t code_stride(const Tensor &t, const char *name, at::Device device, int64_t rows, int64_t cols) {
   int64_t ld = row_stride(t, name, device, ScalarType::Char, rows, cols);
-  if (t.size(0) == 1) ld = (ld + 15) / 16 * 16;  // one row needs no stride of its own
+  if (t.size(0) <= 1) ld = (ld + 15) / 16 * 16;  // one row, or none, needs no stride of its own
   TORCH_CHECK_VALUE(reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && ld % 16 == 0, name,
                     ": int8 rows must start on 16-byte boundaries (row stride ", ld,
                     "); rms_norm and quantize_int8 return them so, weights are laid out once with a padded row stride");
