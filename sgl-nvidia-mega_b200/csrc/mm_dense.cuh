@@ -53,10 +53,24 @@ __device__ __forceinline__ float int8_scale(uint32_t top) {
 // Scales below this (zero and NaN too) take int8_code_tiny.
 constexpr float kTinyScale = 0x1p-120f;
 
-// Whether two ranges of bytes share memory; null pointers do not.
-inline bool overlap(const void *p, int64_t p_bytes, const void *q, int64_t q_bytes) {
-  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
-  return p && q && a < b + q_bytes && b < a + p_bytes;
+// A buffer's bytes: rows of row_bytes, pitch apart (one row: any pitch).
+struct Bytes {
+  const void *p;
+  int64_t rows, row_bytes, pitch;
+};
+inline Bytes row_bytes(const void *p, int64_t rows, int64_t cols, int64_t ld, int size) { return {p, rows, cols * size, ld * size}; }
+inline Bytes flat_bytes(const void *p, int64_t bytes) { return {p, 1, bytes, bytes}; }
+// Whether two buffers share memory; null pointers do not, nor do columns beside each other of
+// rows of one pitch.
+inline bool overlap(const Bytes &a, const Bytes &b) {
+  if (!a.p || !b.p) return false;
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+  if (pa >= pb + ((b.rows - 1) * b.pitch + b.row_bytes) || pb >= pa + ((a.rows - 1) * a.pitch + a.row_bytes)) return false;
+  if (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch) return true;
+  const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+  int64_t from = static_cast<int64_t>(pb - pa) % pitch;  // b's first column among a's
+  if (from < 0) from += pitch;
+  return from < a.row_bytes || from + b.row_bytes > pitch;
 }
 
 // int8 codes and fp32 scales of rows (mm_norm.cu); returns an MM_* status.

@@ -802,9 +802,10 @@ int check(const char *what, const Product &q) {
     return set_error(MM_ERR_INVALID, "%s: a misaligned pointer", what);
   const int es = q.out_type == MM_DTYPE_FP32 ? 4 : 2;
   const int64_t w_rows = q.gated ? 2 * static_cast<int64_t>(q.features) : q.features;
-  auto written = [&](const void *p, int64_t bytes) { return overlap(q.out, ((q.tokens - 1) * q.ld_out + q.features) * es, p, bytes); };
-  if (written(q.x, (q.tokens - 1) * q.ld_x + q.depth) || written(q.w, (w_rows - 1) * q.ld_w + q.depth) ||
-      written(q.x_scale, q.tokens * 4ll) || written(q.w_scale, w_rows * 4) || written(q.bias, q.features * 4ll))
+  auto written = [&](const Bytes &b) { return overlap(row_bytes(q.out, q.tokens, q.features, q.ld_out, es), b); };
+  if (written(row_bytes(q.x, q.tokens, q.depth, q.ld_x, 1)) || written(row_bytes(q.w, w_rows, q.depth, q.ld_w, 1)) ||
+      written(flat_bytes(q.x_scale, q.tokens * 4ll)) || written(flat_bytes(q.w_scale, w_rows * 4)) ||
+      written(flat_bytes(q.bias, q.features * 4ll)))
     return set_error(MM_ERR_INVALID, "%s: the output overlaps an input", what);
   return MM_OK;
 }
@@ -924,18 +925,15 @@ int mm_int8_ffn(const mm_int8_ffn_args *f, void *stream) {
   int rc = check("mm_int8_ffn", up_q);
   if (!rc) rc = check("mm_int8_ffn", down_q);
   if (rc || f->tokens == 0) return rc;
-  struct Buffer {
-    const void *p;
-    int64_t bytes;
-  };
-  const Buffer first[] = {{f->x, (f->tokens - 1) * f->ld_x + f->hidden}, {f->w13, (2ll * f->inter - 1) * f->ld_w13 + f->hidden},
-                          {f->x_scale, f->tokens * 4ll}, {f->w13_scale, f->inter * 8ll}};
-  const Buffer second[] = {{f->w2, (f->hidden - 1) * f->ld_w2 + f->inter}, {f->w2_scale, f->hidden * 4ll}};
-  const int64_t out_bytes = ((f->tokens - 1) * f->ld_out + f->hidden) * (f->out_dtype == MM_DTYPE_FP32 ? 4 : 2);
-  auto in_workspace = [&](const Buffer &b) { return overlap(ws, mm_int8_ffn_workspace(f->tokens, f->inter), b.p, b.bytes); };
-  for (const Buffer &b : first)  // the down product's own check covers second
-    if (overlap(f->out, out_bytes, b.p, b.bytes)) return set_error(MM_ERR_INVALID, "mm_int8_ffn: the output overlaps an input");
-  if (std::any_of(first, first + 4, in_workspace) || std::any_of(second, second + 2, in_workspace) || in_workspace({f->out, out_bytes}))
+  const Bytes first[] = {row_bytes(f->x, f->tokens, f->hidden, f->ld_x, 1), row_bytes(f->w13, 2ll * f->inter, f->hidden, f->ld_w13, 1),
+                         flat_bytes(f->x_scale, f->tokens * 4ll), flat_bytes(f->w13_scale, f->inter * 8ll)};
+  const Bytes second[] = {row_bytes(f->w2, f->hidden, f->inter, f->ld_w2, 1), flat_bytes(f->w2_scale, f->hidden * 4ll)};
+  const Bytes out = row_bytes(f->out, f->tokens, f->hidden, f->ld_out, f->out_dtype == MM_DTYPE_FP32 ? 4 : 2);
+  const Bytes space = flat_bytes(ws, mm_int8_ffn_workspace(f->tokens, f->inter));
+  auto in_workspace = [&](const Bytes &b) { return overlap(space, b); };
+  for (const Bytes &b : first)  // the down product's own check covers second
+    if (overlap(out, b)) return set_error(MM_ERR_INVALID, "mm_int8_ffn: the output overlaps an input");
+  if (std::any_of(first, first + 4, in_workspace) || std::any_of(second, second + 2, in_workspace) || in_workspace(out))
     return set_error(MM_ERR_INVALID, "mm_int8_ffn: the workspace overlaps a buffer");
   if ((rc = run("mm_int8_ffn", up_q, stream))) return rc;
   if ((rc = quantize_rows("mm_int8_ffn", h, ld_h, MM_DTYPE_FP32, hq, ld_q, hs, f->tokens, f->inter, stream))) return rc;

@@ -817,25 +817,20 @@ int run_norm(const char *what, NormArgs a, int dtype, int quant, void *stream) {
   const int es = dtype_bytes(dtype);
   // each thread writes the residual over elements that it alone has read, so that it may take
   // x's or the residual's own place, row for row; no other buffers may share memory with an output
-  struct Buffer {
-    const void *p;
-    int64_t bytes;
-  };
-  auto rows = [&](const void *p, int64_t ld, int size) { return Buffer{p, ((a.tokens - 1) * ld + a.hidden) * size}; };
-  const Buffer in[] = {rows(a.x, a.ld_x, es), rows(a.residual, a.ld_residual, es),
-                       {a.gamma, static_cast<int64_t>(a.hidden) * (a.gamma_f32 ? 4 : es)}};
+  auto rows = [&](const void *p, int64_t ld, int size) { return row_bytes(p, a.tokens, a.hidden, ld, size); };
+  const Bytes in[] = {rows(a.x, a.ld_x, es), rows(a.residual, a.ld_residual, es),
+                      flat_bytes(a.gamma, static_cast<int64_t>(a.hidden) * (a.gamma_f32 ? 4 : es))};
   const int64_t scale_bytes = quant == MM_QUANT_MXFP8 ? static_cast<int64_t>(a.tokens) * (a.hidden / 32) : static_cast<int64_t>(a.tokens) * 4;
-  const Buffer out[] = {rows(a.residual_out, a.ld_residual_out, es), rows(a.norm_out, a.ld_norm, es),
-                        rows(quant ? a.codes : nullptr, a.ld_codes, 1), {quant ? a.scales : nullptr, scale_bytes}};
-  auto in_place = [&](const Buffer &o, const Buffer &i) {
+  const Bytes out[] = {rows(a.residual_out, a.ld_residual_out, es), rows(a.norm_out, a.ld_norm, es),
+                       rows(quant ? a.codes : nullptr, a.ld_codes, 1), flat_bytes(quant ? a.scales : nullptr, scale_bytes)};
+  auto in_place = [&](const Bytes &o, const Bytes &i) {
     return &o == out && o.p == i.p && ((&i == in && a.ld_x == a.ld_residual_out) || (&i == in + 1 && a.ld_residual == a.ld_residual_out));
   };
-  for (const Buffer &o : out) {
-    for (const Buffer &i : in)
-      if (overlap(o.p, o.bytes, i.p, i.bytes) && !in_place(o, i))
-        return set_error(MM_ERR_INVALID, "%s: an output overlaps an input", what);
-    for (const Buffer &other : out)
-      if (&other < &o && overlap(o.p, o.bytes, other.p, other.bytes)) return set_error(MM_ERR_INVALID, "%s: an output overlaps another", what);
+  for (const Bytes &o : out) {
+    for (const Bytes &i : in)
+      if (overlap(o, i) && !in_place(o, i)) return set_error(MM_ERR_INVALID, "%s: an output overlaps an input", what);
+    for (const Bytes &other : out)
+      if (&other < &o && overlap(o, other)) return set_error(MM_ERR_INVALID, "%s: an output overlaps another", what);
   }
   const uintptr_t base = reinterpret_cast<uintptr_t>(a.x);
   bool wide = true;

@@ -14,7 +14,8 @@ Every call runs on the current stream of the tensors' device, allocates its
 outputs and its workspace from torch's allocator (so calls on several streams,
 and captured graphs, share none) and never synchronizes. Tensors are 2-D with
 their last dimension contiguous; rows may be strided. An output given as ``out=``
-may not share memory with an input (``rms_norm``'s ``residual_out`` may). Outputs of
+may not share memory with an input (``rms_norm``'s ``residual_out`` may; columns beside
+each other of one buffer's rows share none). Outputs of
 one call of up to 1 MiB together are parts of one allocation, which lives as long as
 any of them. The operators are for inference: outputs carry no gradient. Violations
 raise ValueError.
