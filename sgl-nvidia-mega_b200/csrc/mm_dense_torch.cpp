@@ -70,6 +70,11 @@ struct Args {
     TORCH_CHECK_TYPE(i < n && THPDtype_Check(v[i]), name, " must be a torch.dtype");
     return reinterpret_cast<THPDtype *>(v[i])->scalar_type;
   }
+  bool truth(int i) const {
+    const int t = PyObject_IsTrue(v[i]);
+    if (t < 0) throw python_error();
+    return t == 1;
+  }
   double number(int i, const char *name) const {
     TORCH_CHECK_TYPE(i < n, name, " is missing");
     const double d = PyFloat_AsDouble(v[i]);
@@ -193,7 +198,7 @@ PyObject *rms_norm(PyObject *, PyObject *const *v, Py_ssize_t n) {
   m.x = x.data_ptr();
   m.tokens = static_cast<int32_t>(tokens);
   m.hidden = static_cast<int32_t>(hidden);
-  const bool has_with = a.has(5), with = has_with && PyObject_IsTrue(v[5]) == 1;
+  const bool has_with = a.has(5), with = has_with && a.truth(5);
   const bool wants_norm = m.quant == MM_QUANT_NONE || with || a.has(6);
   TORCH_CHECK_VALUE(!(wants_norm && has_with && !with), "with_norm=False needs quant and no out");
   TORCH_CHECK_VALUE(a.has(3) || !a.has(7), "residual_out needs residual");

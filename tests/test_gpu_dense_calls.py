@@ -78,3 +78,13 @@ def test_columns_that_meet_are_refused(first):
     x, out = (room[at:].as_strided((4, 512), (1024, 1)) for at in (0, first))
     with pytest.raises(ValueError, match="overlaps"):
         megamoe.rms_norm(x, torch.ones(512, dtype=BF, device="cuda"), out=out)
+
+
+def test_an_error_in_an_argument_reaches_the_caller():
+    class Undecided:
+        def __bool__(self):
+            raise KeyError("undecided")
+
+    x, gamma = torch.ones((2, 64), dtype=BF, device="cuda"), torch.ones(64, dtype=BF, device="cuda")
+    with pytest.raises(KeyError, match="undecided"):
+        megamoe.rms_norm(x, gamma, quant="int8", with_norm=Undecided())
