@@ -63,14 +63,35 @@ def _older(output: str, deps) -> bool:
     return not os.path.exists(output) or any(os.path.getmtime(p) > os.path.getmtime(output) for p in deps)
 
 
+def _own() -> list:
+    return [os.path.join(REPO, "include", "megamoe.h"), os.path.abspath(__file__)]
+
+
 def _stale() -> bool:
-    own = [os.path.join(REPO, "include", "megamoe.h"), os.path.abspath(__file__)]
-    return _older(OUTPUT, [os.path.join(CSRC, f) for f in SOURCES + HEADERS] + own) or _torch_stale()
+    return _older(OUTPUT, [os.path.join(CSRC, f) for f in SOURCES + HEADERS] + _own())
+
+
+def _torch_abi() -> str:
+    """What _dense.so is compiled against: it loads beside no other."""
+    import sysconfig
+
+    import torch
+
+    return f"{sysconfig.get_config_var('SOABI')} torch {torch.__version__} {torch.__file__} cxx11 {int(torch.compiled_with_cxx11_abi())}"
+
+
+def _torch_stamp() -> str:
+    return os.path.join(OBJDIR, "_dense.abi")
 
 
 def _torch_stale() -> bool:
-    return _older(TORCH_OUTPUT, [os.path.join(CSRC, TORCH_SOURCE), os.path.join(REPO, "include", "megamoe.h"),
-                                 os.path.abspath(__file__)])
+    if _older(TORCH_OUTPUT, [os.path.join(CSRC, TORCH_SOURCE)] + _own()):
+        return True
+    try:
+        with open(_torch_stamp()) as f:
+            return f.read() != _torch_abi()
+    except OSError:
+        return True
 
 
 def _run(cmd, verbose):
@@ -81,9 +102,16 @@ def _run(cmd, verbose):
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    """Compile the library if any source is newer than it; returns its path."""
-    if not force and not _stale():
-        return OUTPUT
+    """Compile the library, and the binding of the dense operators, where a source is newer
+    than they are (the binding: or where torch or Python is another); returns the library's path."""
+    if force or _stale():
+        _build_library(verbose)
+    if force or _torch_stale():
+        _build_binding(verbose)
+    return OUTPUT
+
+
+def _build_library(verbose: bool) -> None:
     os.makedirs(OBJDIR, exist_ok=True)
     objs = [os.path.join(OBJDIR, s.replace(".cu", ".o")) for s in SOURCES]
     cmds = [[NVCC, *compile_flags(s), *(["-Xptxas", "-v"] if verbose else []), "-c", os.path.join(CSRC, s), "-o", o]
@@ -99,13 +127,17 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)
         raise RuntimeError(f"nvcc link failed ({res.returncode}) building {OUTPUT}")
-    if force or _torch_stale():
-        cmd = torch_command()
-        res = _run(cmd, verbose)
-        if res.returncode != 0:
-            sys.stderr.write(res.stdout + res.stderr)
-            raise RuntimeError(f"g++ failed ({res.returncode}): {' '.join(cmd)}")
-    return OUTPUT
+
+
+def _build_binding(verbose: bool) -> None:
+    cmd = torch_command()
+    res = _run(cmd, verbose)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout + res.stderr)
+        raise RuntimeError(f"g++ failed ({res.returncode}): {' '.join(cmd)}")
+    os.makedirs(OBJDIR, exist_ok=True)
+    with open(_torch_stamp(), "w") as f:
+        f.write(_torch_abi())
 
 
 if __name__ == "__main__":
