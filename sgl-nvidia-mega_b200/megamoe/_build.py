@@ -10,6 +10,7 @@ options for that gate), every other file the default IEEE ones.
 from __future__ import annotations
 
 import os
+import shutil
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -38,18 +39,26 @@ def compile_flags(source: str) -> list:
     return [*COMPILE, *FILE_FLAGS.get(source, []), "-I", os.path.join(REPO, "include"), "-I", CSRC]
 
 
-def torch_command() -> list:
-    """g++ command that builds _dense.so against the running Python and torch."""
+def _torch_headers() -> dict:
+    """The include folders of _dense.so: a header that each has to hold, and where."""
     import sysconfig
 
+    import torch
+
+    include = os.path.join(os.path.dirname(torch.__file__), "include")
+    return {"Python.h": sysconfig.get_paths()["include"], "torch/csrc/Dtype.h": include,
+            "torch/torch.h": os.path.join(include, "torch", "csrc", "api", "include"),
+            "cuda_runtime_api.h": os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")}
+
+
+def torch_command() -> list:
+    """g++ command that builds _dense.so against the running Python and torch."""
     import torch
 
     root = os.path.dirname(torch.__file__)
     lib = os.path.join(root, "lib")
     abi = int(torch.compiled_with_cxx11_abi())
-    includes = [os.path.join(REPO, "include"), sysconfig.get_paths()["include"], os.path.join(root, "include"),
-                os.path.join(root, "include", "torch", "csrc", "api", "include"),
-                os.path.join(os.path.dirname(os.path.dirname(NVCC)), "include")]
+    includes = [os.path.join(REPO, "include"), *_torch_headers().values()]
     return [CXX, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *(f"-I{i}" for i in includes),
             os.path.join(CSRC, TORCH_SOURCE), "-o", TORCH_OUTPUT, f"-L{HERE}", "-l:libmegamoe.so", "-Wl,-rpath,$ORIGIN",
             f"-L{lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
@@ -130,6 +139,15 @@ def _build_library(verbose: bool) -> None:
 
 
 def _build_binding(verbose: bool) -> None:
+    missing = [h for h, folder in _torch_headers().items() if not os.path.exists(os.path.join(folder, h))]
+    missing += [] if shutil.which(CXX) else [CXX]
+    if missing:
+        # the library and its MoE chain need none of them; the dense operators' calls will say
+        # that _dense.so is not there, so one built for something else must not be
+        if os.path.exists(TORCH_OUTPUT):
+            os.remove(TORCH_OUTPUT)
+        sys.stderr.write(f"megamoe: _dense.so is left out, the dense operators cannot be called: no {', '.join(missing)} here\n")
+        return
     cmd = torch_command()
     res = _run(cmd, verbose)
     if res.returncode != 0:

@@ -74,3 +74,37 @@ def test_the_binding_is_built_again_for_another_torch_or_python(tree, monkeypatc
     tree.commands.clear()
     _build.build()
     assert tree.commands == []
+
+
+def test_a_host_without_the_headers_still_builds_the_library(tree, monkeypatch, tmp_path, capsys):
+    """Python.h missing: the library (the MoE chain) is built, the binding is named as left out,
+    and one compiled for other headers does not stay behind to be loaded."""
+    import sysconfig
+
+    real = sysconfig.get_paths
+    monkeypatch.setattr(sysconfig, "get_paths", lambda *a, **k: dict(real(*a, **k), include=str(tmp_path / "none")))
+    assert _build.build(force=True) == _build.OUTPUT
+    assert "libmegamoe.so" in tree.outputs() and "_dense.so" not in tree.outputs()
+    assert not os.path.exists(_build.TORCH_OUTPUT)
+    err = capsys.readouterr().err
+    assert "_dense.so" in err and "Python.h" in err
+
+
+def test_a_compiler_error_is_an_error(tree, monkeypatch):
+    monkeypatch.setattr(_build, "_run", lambda cmd, verbose: subprocess.CompletedProcess(cmd, 1, "", "no"))
+    os.remove(_build.TORCH_OUTPUT)
+    with pytest.raises(RuntimeError, match="g\\+\\+ failed"):
+        _build.build()
+
+
+def test_calls_without_the_binding_say_what_is_missing(monkeypatch):
+    import sys
+
+    import megamoe
+    from megamoe import dense
+
+    monkeypatch.setattr(dense, "_dense", None)
+    monkeypatch.setitem(sys.modules, "megamoe._dense", None)
+    monkeypatch.delattr(megamoe, "_dense", raising=False)
+    with pytest.raises(RuntimeError, match="_dense.so does not load"):
+        megamoe.quantize_int8(None)
