@@ -347,6 +347,16 @@ int mm_int8_ffn(const mm_int8_ffn_args *args, void *stream);
  * products' bounded waits on it: MM_OK or MM_ERR_DEVICE_TIMEOUT. */
 int mm_int8_check(void);
 
+/* The budget of every bounded wait of the int8 products that this process launches or
+ * captures from now on, 1 us .. 60 s (default 1.5 s). */
+int mm_int8_set_wait_budget(int64_t microseconds);
+
+/* A test hook for the timeout path: in each of the next `launches` int8 products of this
+ * process, the CTAs of that rank in their cluster (0..7; few tokens) or pair (0..1; many
+ * tokens) leave out the last load of their (first) tile, so that the wait for it runs out,
+ * the launch ends and mm_int8_check reports MM_ERR_DEVICE_TIMEOUT. */
+int mm_int8_withhold(int32_t rank, int32_t launches);
+
 /* ---- combine + all-reduce over NVLink peer memory ------------------------ */
 /* One rank's view of a TP/EP group whose ranks exchange their partial outputs
  * by plain P2P stores into each other's buffers (CUDA IPC; no multicast). */

@@ -21,6 +21,7 @@
 // 128 rows of the stream form (they meet in shared memory, where its parts are added anyway),
 // 128 and 128 as the two halves of the tile form's columns (one TMEM lane then holds both).
 #include <algorithm>
+#include <atomic>
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -63,6 +64,8 @@ struct alignas(64) Int8Args {
   int token_tiles, feature_tiles, tile_n;  // of the tile form
   int w_early;          // the launch's predecessors do not write the weights: load before waiting
   int split;            // CTAs of a cluster that share a tile's depth (stream form), a power of two
+  int withhold;         // mm_int8_withhold: this rank's CTAs leave out a load; -1: none
+  uint64_t wait_ns;     // budget of every bounded wait (mm_int8_set_wait_budget)
 };
 
 // A whole warp waits, one elected lane issues: the lanes go on together, or give up together.
@@ -203,17 +206,18 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
       for (int a = 0; a < kRowsM / S::kFeatures; ++a)
         tma_load_3d(stage + a * S::kFeatures * kBlockK, &p.w_map, (kb0 + i) * kBlockK, f0, a, bar, gridDim.y > 1 ? keep : stream_once);
     };
-    const int early = p.w_early ? min(n, S::kStages) : 0;
+    const int loads = n - (p.withhold == rank ? 1 : 0);
+    const int early = p.w_early ? min(loads, S::kStages) : 0;
     if (elect_one())
       for (int i = 0; i < early; ++i) load_w(i);
     __syncwarp();
     pdl_wait();
     pdl_launch_dependents();
     int i = 0;
-    for (; i < n; ++i) {
+    for (; i < loads; ++i) {
       const int s = i % S::kStages;
       if (i >= S::kStages &&
-          !warp_agrees(mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty)))
+          !warp_agrees(mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty, p.wait_ns)))
         break;
       if (elect_one()) {
         if (i >= early) load_w(i);
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
     constexpr uint32_t idesc = idesc_i8(kRowsM, BN);
     for (int i = 0; i < n; ++i) {
       const int s = i % S::kStages;
-      if (!warp_agrees(mbar_wait(full + 8 * s, (i / S::kStages) & 1, &g_int8_error, kErrTimeoutFull))) {
+      if (!warp_agrees(mbar_wait(full + 8 * s, (i / S::kStages) & 1, &g_int8_error, kErrTimeoutFull, p.wait_ns))) {
         *failed = 1u;
         break;
       }
@@ -263,7 +267,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
     second[i] = i >= left ? 0.0f : GATED ? p.w_scale[static_cast<int64_t>(p.features) + f + i] : p.bias ? p.bias[f + i] : 0.0f;
   }
   if (warp >= 2 && threadIdx.x - 64 < live) x_scale[threadIdx.x - 64] = p.x_scale[t0 + threadIdx.x - 64];
-  bool ok = mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc);
+  bool ok = mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc, p.wait_ns);
   tc_fence_after();
   ok = ok && *failed == 0u;
   // Every CTA of the cluster finishes the tokens rank, rank + split, ... Groups of four warps read the
@@ -310,7 +314,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
     tc_fence_before();
     __syncthreads();  // x's scales, and the TMEM reads
     if (warp == 1) tmem_dealloc(tmem, S::kCols);
-    if (rank < live && !mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc)) {
+    if (rank < live && !mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc, p.wait_ns)) {
       cluster_sync();  // parts may still come: stay until their senders are gone
       return;
     }
@@ -453,9 +457,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       const int t0 = tt * kTileM + rank * kRowsM;
       const int row = GATED ? ft * tile_f : ft * tile_f + rank * half_n, plane = GATED ? rank : 0;
       for (int kb = 0; kb < p.blocks_k; kb += kTileBlocks, ++it) {
+        if (p.withhold == rank && kb + kTileBlocks >= p.blocks_k) {  // of the first tile
+          ok = false;
+          break;
+        }
         const int s = it % kTileStages;
         if (it >= kTileStages &&
-            !warp_agrees(mbar_wait_cluster(empty + 8 * s, ((it / kTileStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty))) {
+            !warp_agrees(mbar_wait_cluster(empty + 8 * s, ((it / kTileStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty, p.wait_ns))) {
           ok = false;
           break;
         }
@@ -475,9 +483,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       }
     }
     // leave no copy in flight: the last stages' barriers complete with both CTAs' copies
-    if (rank == 0)
+    if (rank == 0) {
       for (int j = max(0, it - kTileStages); j < it; ++j)
         mbar_wait_drain(full + 8 * (j % kTileStages), (j / kTileStages) & 1);
+    } else if (!ok) {
+      // the leader may have stopped before this CTA did, and then has not waited for all of its copies
+      for (const uint64_t t0 = globaltimer(); globaltimer() - t0 < kDrainBudgetNs;) {}
+    }
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0) {
@@ -486,11 +498,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += pairs, ++n) {
         const int b = n & 1;
-        if (n >= 2 && !warp_agrees(mbar_wait_cluster(acc_empty + 8 * b, ((n >> 1) - 1) & 1, &g_int8_error, kErrTimeoutAcc))) break;
+        if (n >= 2 && !warp_agrees(mbar_wait_cluster(acc_empty + 8 * b, ((n >> 1) - 1) & 1, &g_int8_error, kErrTimeoutAcc, p.wait_ns))) break;
         tc_fence_after();
         for (int kb = 0; kb < p.blocks_k; kb += kTileBlocks, ++it) {
           const int s = it % kTileStages;
-          if (!warp_agrees(mbar_wait_cluster(full + 8 * s, (it / kTileStages) & 1, &g_int8_error, kErrTimeoutFull))) {
+          if (!warp_agrees(mbar_wait_cluster(full + 8 * s, (it / kTileStages) & 1, &g_int8_error, kErrTimeoutFull, p.wait_ns))) {
             ok = false;
             break;
           }
@@ -554,7 +566,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       }
       __syncwarp();
       if (tile + pairs < tiles) fetch(tile + pairs);
-      if (!warp_agrees(mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc))) break;
+      if (!warp_agrees(mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc, p.wait_ns))) break;
       tc_fence_after();
       const uint32_t from = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kTileN;
       for (int c = half * CH, i0 = 0; c < tile_f; c += 2 * CH, i0 += CH) {
@@ -707,6 +719,16 @@ cudaError_t launch_cluster(K kernel, dim3 grid, int threads, int smem, int clust
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+// The budget of the bounded waits, and what mm_int8_withhold asked for: of this process's launches.
+std::atomic<int64_t> g_wait_ns{static_cast<int64_t>(kWaitBudgetNs)};
+std::atomic<int> g_withhold_rank{0}, g_withhold_launches{0};
+
+int withheld() {
+  for (int n = g_withhold_launches.load(); n > 0;)
+    if (g_withhold_launches.compare_exchange_weak(n, n - 1)) return g_withhold_rank.load();
+  return -1;
+}
+
 // CTAs of a cluster that share a tile's depth: enough CTAs for most SMs, each with at least two
 // blocks of depth.
 int stream_split(int64_t tiles, int blocks_k) {
@@ -824,6 +846,8 @@ int run(const char *what, const Product &q, void *stream) {
   a.has_clamp = q.clamp > 0.0f;
   a.clamp = q.clamp;
   a.w_early = q.w_early;
+  a.wait_ns = static_cast<uint64_t>(g_wait_ns.load());
+  a.withhold = withheld();
   auto w_map = [&](int rows) { return encode(&a.w_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.w, q.depth, q.features, q.gated ? 2 : 1, q.ld_w, rows); };
   int rc;
   auto x_map = [&](int rows) { return encode(&a.x_map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, q.x, q.depth, q.tokens, 0, q.ld_x, rows); };
@@ -938,6 +962,20 @@ int mm_int8_ffn(const mm_int8_ffn_args *f, void *stream) {
   if ((rc = run("mm_int8_ffn", up_q, stream))) return rc;
   if ((rc = quantize_rows("mm_int8_ffn", h, ld_h, MM_DTYPE_FP32, hq, ld_q, hs, f->tokens, f->inter, stream))) return rc;
   return run("mm_int8_ffn", down_q, stream);
+}
+
+int mm_int8_set_wait_budget(int64_t microseconds) {
+  if (microseconds < 1 || microseconds > 60000000)
+    return set_error(MM_ERR_INVALID, "mm_int8_set_wait_budget: %lld us outside 1..60000000", static_cast<long long>(microseconds));
+  g_wait_ns.store(microseconds * 1000);
+  return MM_OK;
+}
+
+int mm_int8_withhold(int32_t rank, int32_t launches) {
+  if (rank < 0 || rank > 7 || launches < 0) return set_error(MM_ERR_INVALID, "mm_int8_withhold: rank %d, %d launches", rank, launches);
+  g_withhold_rank.store(rank);
+  g_withhold_launches.store(launches);
+  return MM_OK;
 }
 
 int mm_int8_check(void) {

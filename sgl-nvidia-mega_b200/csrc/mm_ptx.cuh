@@ -21,8 +21,8 @@ constexpr uint32_t kErrBadUnit = 1u << 8;        // a work item failed its check
 constexpr uint32_t kErrTimeoutMask = 0xffu;
 
 // The default budget of one bounded wait, 1.5 s: far above any legitimate wait
-// of one launch, far below any watchdog. Layers and comms carry their own budget
-// (mm_layer_set_wait_budget / mm_comm_set_wait_budget), passed to every wait.
+// of one launch, far below any watchdog. Layers, comms and the int8 products carry their
+// own budget (mm_layer_ / mm_comm_ / mm_int8_set_wait_budget), passed to every wait.
 constexpr uint64_t kWaitBudgetNs = 1500000000ull;
 // The limit of a teardown drain (copies and MMAs this CTA issued, which complete
 // in microseconds); a drain ignores the error word, so a launch that gave up
@@ -406,7 +406,8 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
       : "memory");
   return ok != 0u;
 }
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint32_t *err, uint32_t code) {
+__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint32_t *err, uint32_t code,
+                                                  uint64_t budget_ns = kWaitBudgetNs) {
 #pragma unroll 1
   for (int i = 0; i < 256; ++i)
     if (mbar_try_wait_cluster(bar, parity)) return true;
@@ -416,7 +417,7 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity,
     if (mbar_try_wait_cluster(bar, parity)) return true;
     if ((i & 63u) == 0u) {
       if (error_set(err)) return false;
-      if (globaltimer() - t0 > kWaitBudgetNs) {
+      if (globaltimer() - t0 > budget_ns) {
         error_raise(err, code);
         return false;
       }

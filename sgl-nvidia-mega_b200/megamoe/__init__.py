@@ -17,9 +17,9 @@ from .moe import (  # noqa: F401
     route_words,
     router_gemv,
 )
-from .dense import NormOutput, int8_check, int8_ffn, int8_linear, quantize_int8, rms_norm  # noqa: F401
+from .dense import NormOutput, int8_check, int8_ffn, int8_linear, int8_set_wait_budget, quantize_int8, rms_norm  # noqa: F401
 from .comm import PeerAllReduce  # noqa: F401
 from .stack import MoEStack  # noqa: F401
 
 __all__ = ["MoEStack", "NormOutput", "PeerAllReduce", "RoutedMoE", "finalize", "finalize_partial", "gate_topk", "int8_check",
-           "int8_ffn", "int8_linear", "quantize_int8", "rms_norm", "route", "route_words", "router_gemv"]
+           "int8_ffn", "int8_linear", "int8_set_wait_budget", "quantize_int8", "rms_norm", "route", "route_words", "router_gemv"]

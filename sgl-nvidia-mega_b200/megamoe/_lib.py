@@ -231,6 +231,8 @@ SIGNATURES = {
     "mm_int8_ffn_workspace": (c_int64, [c_int32, c_int32]),
     "mm_int8_ffn": (c_int32, [POINTER(MMInt8FFNArgs), c_void_p]),
     "mm_int8_check": (c_int32, []),
+    "mm_int8_set_wait_budget": (c_int32, [c_int64]),
+    "mm_int8_withhold": (c_int32, [c_int32, c_int32]),
     "mm_finalize": (
         c_int32,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p],

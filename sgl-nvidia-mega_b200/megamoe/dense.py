@@ -107,3 +107,9 @@ def int8_check(device: Optional[torch.device] = None) -> None:
     ``int8_linear`` or ``int8_ffn`` gave up on this device (default: the current one)."""
     with torch.cuda.device(device):
         check(lib().mm_int8_check(), "int8_check")
+
+
+def int8_set_wait_budget(microseconds: int) -> None:
+    """Budget of every bounded device wait of the int8 products that this process launches or
+    captures from now on (default 1.5 s)."""
+    check(lib().mm_int8_set_wait_budget(int(microseconds)), "int8_set_wait_budget")

@@ -1,0 +1,69 @@
+"""Bounded waits of the int8 products that run out: the launch ends within its budget,
+int8_check raises, and the next call is right again. Each test makes a wait run out on a load
+that is left out (mm_int8_withhold), with a short budget; no kernel waits without a bound."""
+
+import time
+
+import pytest
+import torch
+
+import megamoe
+from megamoe import _lib
+
+pytestmark = pytest.mark.gpu
+
+BUDGET_US = 5000
+# (tokens, features, depth, ranks): one CTA a tile; parts sent to, and read by, eight CTAs; pairs
+FORMS = [(3, 40000, 1024, (0,)), (4, 300, 7168, (0, 1, 7)), (30, 130, 4096, (0, 3)), (80, 300, 7168, (0, 5)), (128, 256, 4096, (7,)),
+         (600, 1000, 2048, (0, 1)), (4096, 4096, 512, (0, 1))]
+
+
+def operands(tokens, features, depth):
+    g = torch.Generator(device="cuda").manual_seed(tokens + features)
+    x, w = (torch.randint(-127, 128, (n, depth), dtype=torch.int8, device="cuda", generator=g) for n in (tokens, features))
+    return x, torch.full((tokens,), 2.0 ** -8, device="cuda"), w, torch.full((features,), 2.0 ** -8, device="cuda")
+
+
+@pytest.fixture(autouse=True)
+def settings():
+    megamoe.int8_check()
+    megamoe.int8_set_wait_budget(BUDGET_US)
+    yield
+    _lib.lib().mm_int8_withhold(0, 0)
+    megamoe.int8_set_wait_budget(1_500_000)
+    torch.cuda.synchronize()
+    try:
+        megamoe.int8_check()
+    except _lib.DeviceTimeoutError:
+        pass
+
+
+@pytest.mark.parametrize("tokens,features,depth,ranks", FORMS)
+def test_a_wait_runs_out_and_the_next_call_is_right(tokens, features, depth, ranks):
+    call = operands(tokens, features, depth)
+    want = megamoe.int8_linear(*call)
+    megamoe.int8_check()
+    for rank in ranks:
+        _lib.lib().mm_int8_withhold(rank, 1)
+        t0 = time.perf_counter()
+        megamoe.int8_linear(*call)
+        with pytest.raises(_lib.DeviceTimeoutError):
+            megamoe.int8_check()
+        # the budget and the teardown's drains (20 ms at most each), far below the default of 1.5 s
+        assert time.perf_counter() - t0 < 1.0
+        got = megamoe.int8_linear(*call)
+        megamoe.int8_check()
+        assert torch.equal(got, want)
+
+
+def test_a_wait_of_the_block_runs_out():
+    x, xs, w13, s13 = operands(20, 1024, 512)
+    _, _, w2, s2 = operands(1, 512, 512)
+    want = megamoe.int8_ffn(x, xs, w13, s13, w2, s2)
+    for launches in (1, 2):
+        _lib.lib().mm_int8_withhold(0, launches)
+        megamoe.int8_ffn(x, xs, w13, s13, w2, s2)
+        with pytest.raises(_lib.DeviceTimeoutError):
+            megamoe.int8_check()
+        assert torch.equal(megamoe.int8_ffn(x, xs, w13, s13, w2, s2), want)
+        megamoe.int8_check()
