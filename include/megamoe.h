@@ -344,7 +344,8 @@ int64_t mm_int8_ffn_workspace(int32_t tokens, int32_t inter);
 int mm_int8_ffn(const mm_int8_ffn_args *args, void *stream);
 
 /* Synchronizes the current device and reads (then clears) the error word of the int8
- * products' bounded waits on it: MM_OK or MM_ERR_DEVICE_TIMEOUT. */
+ * products' bounded waits on it: MM_OK or MM_ERR_DEVICE_TIMEOUT. A launch whose wait ran
+ * out writes NaN where its sums are not whole. */
 int mm_int8_check(void);
 
 /* The budget of every bounded wait of the int8 products that this process launches or

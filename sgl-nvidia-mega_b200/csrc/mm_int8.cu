@@ -45,6 +45,10 @@ constexpr int kTileTokens = 128;
 constexpr double kTileUs = 4.0, kTileColumnUs = 0.346 / 448;  // a launch; a column of a block of depth
 constexpr double kStreamUs = 7.5, kStreamBlockUs = 0.45;      // a round of 128-token CTAs; a block
 
+// In place of a part that a CTA could not compute: parts are sums of at most 2^17 - 1 products
+// of at most 2^14 in magnitude.
+constexpr int kNoPart = INT32_MIN;
+
 // Error word of this file's launches: bounded waits that ran out (mm_int8_check).
 __device__ uint32_t g_int8_error;
 
@@ -234,6 +238,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
       const int s = i % S::kStages;
       if (!warp_agrees(mbar_wait(full + 8 * s, (i / S::kStages) & 1, &g_int8_error, kErrTimeoutFull, p.wait_ns))) {
         *failed = 1u;
+        __threadfence_block();
         break;
       }
       tc_fence_after();
@@ -267,15 +272,15 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
     second[i] = i >= left ? 0.0f : GATED ? p.w_scale[static_cast<int64_t>(p.features) + f + i] : p.bias ? p.bias[f + i] : 0.0f;
   }
   if (warp >= 2 && threadIdx.x - 64 < live) x_scale[threadIdx.x - 64] = p.x_scale[t0 + threadIdx.x - 64];
-  bool ok = mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc, p.wait_ns);
+  const bool ok = warp_agrees(mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc, p.wait_ns) && *failed == 0u);
+  if (!ok) pause_drain();  // copies still in flight land before this CTA's marks below, not over them
   tc_fence_after();
-  ok = ok && *failed == 0u;
   // Every CTA of the cluster finishes the tokens rank, rank + split, ... Groups of four warps read the
   // sums (warp w: TMEM lanes 32 (w % 4) and on, weight rows; a column a token), 16 tokens in turn.
   const int q = warp & 3, group = warp < 2 ? -1 : (warp - 2) >> 2;
   const uint32_t sums = tmem + (static_cast<uint32_t>(q * 32) << 16);
-  auto finish = [&](int j, int4 sum) {
-    const float xs = x_scale[j];
+  auto finish = [&](int j, int4 sum, int least) {
+    const float xs = least != kNoPart ? x_scale[j] : __uint_as_float(0x7fc00000u);  // NaN where a part is missing
     const float a[4] = {__fmul_rn(static_cast<float>(sum.x), xs), __fmul_rn(static_cast<float>(sum.y), xs),
                         __fmul_rn(static_cast<float>(sum.z), xs), __fmul_rn(static_cast<float>(sum.w), xs)};
     float v[PER];
@@ -284,10 +289,24 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
       if constexpr (GATED) v[i] = gate_up(p, __fmul_rn(a[i], ws[i]), __fmul_rn(a[PER + i], second[i]));
       else v[i] = __fmaf_rn(a[i], ws[i], second[i]);
     }
-    if (ok && left > 0) store_some<PER>(p, (t0 + j) * p.ld_out + f, left, v, wide);
+    if (left > 0) store_some<PER>(p, (t0 + j) * p.ld_out + f, left, v, wide);
   };
-  // the four sums of a lane: four features, or two features' gate and up
-  auto add = [](int4 &sum, const int4 &v) { sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w; };
+  // The four sums of a lane: four features, or two features' gate and up. A CTA that gave up leaves
+  // kNoPart, which no part can be, where its sums are missing; neighbours among the four come from
+  // one of its warps, and are missing together.
+  int least;
+  auto add = [&](int4 &sum, const int4 &v) {
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    least = min(least, GATED ? min(v.x, v.z) : v.x);
+  };
+  auto parts = [&](int j, uint32_t (&r)[16]) {
+    tc_ld_32x32b_x16(sums + j, r);
+    tc_wait_ld();
+    if (!ok) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) r[i] = static_cast<uint32_t>(kNoPart);
+    }
+  };
   if (S::kPush && split > 1) {
     // The parts go into the ring of the CTA that finishes their token, once every CTA of the
     // cluster is past its products: [token's turn][part][weight row].
@@ -298,8 +317,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
 #pragma unroll 1
       for (int j = 16 * group; j < live; j += 16 * S::kGroups) {
         uint32_t r[16];
-        tc_ld_32x32b_x16(sums + j, r);
-        tc_wait_ld();
+        parts(j, r);
         if (j == 16 * group) cluster_wait();
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -314,14 +332,13 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
     tc_fence_before();
     __syncthreads();  // x's scales, and the TMEM reads
     if (warp == 1) tmem_dealloc(tmem, S::kCols);
-    if (rank < live && !mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc, p.wait_ns)) {
-      cluster_sync();  // parts may still come: stay until their senders are gone
-      return;
-    }
+    if (rank >= live) return;
+    const bool came = warp_agrees(mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc, p.wait_ns));
 #pragma unroll 1
     for (int j = rank + split * warp; j < live; j += split * S::kWarps) {
       const int *part = reinterpret_cast<const int *>(ring_ptr) + (j & ~(split - 1)) * kRowsM + PER * lane;
       int4 sum = make_int4(0, 0, 0, 0);
+      least = came ? 0 : kNoPart;
 #pragma unroll 8
       for (int r = 0; r < split; ++r, part += kRowsM) {
         if constexpr (GATED) {
@@ -331,8 +348,9 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
           add(sum, *reinterpret_cast<const int4 *>(part));
         }
       }
-      finish(j, sum);
+      finish(j, sum, least);
     }
+    if (!came) cluster_sync();  // parts may still come: stay until their senders are gone
     return;
   }
   // Each CTA leaves its parts in its own ring, [token][weight row], and reads the others' there, from
@@ -341,8 +359,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
 #pragma unroll 1
     for (int j = 16 * group; j < live; j += 16 * S::kGroups) {
       uint32_t r[16];
-      tc_ld_32x32b_x16(sums + j, r);
-      tc_wait_ld();
+      parts(j, r);
       uint32_t *to = reinterpret_cast<uint32_t *>(ring_ptr) + j * kRowsM + q * 32 + lane;
 #pragma unroll
       for (int i = 0; i < 16; ++i) to[i * kRowsM] = r[i];
@@ -355,6 +372,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
   for (int j = rank + split * warp; j < live; j += split * S::kWarps) {
     const uint32_t at = ring + (j * kRowsM + PER * lane) * 4;
     int4 sum = make_int4(0, 0, 0, 0);
+    least = 0;
 #pragma unroll 2
     for (int r = 0; r < split; ++r) {
       const uint32_t from = cluster_map(at, (rank + r) & (split - 1));
@@ -365,7 +383,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
         add(sum, cluster_load_v4(from));
       }
     }
-    finish(j, sum);
+    finish(j, sum, least);
   }
   cluster_sync();  // the parts are read: the CTA may end
 }
@@ -488,7 +506,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
         mbar_wait_drain(full + 8 * (j % kTileStages), (j / kTileStages) & 1);
     } else if (!ok) {
       // the leader may have stopped before this CTA did, and then has not waited for all of its copies
-      for (const uint64_t t0 = globaltimer(); globaltimer() - t0 < kDrainBudgetNs;) {}
+      pause_drain();
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -552,12 +570,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
     };
     if (pair < tiles) fetch(pair);
     int n = 0;
+    bool ok = true;
     for (int tile = pair; tile < tiles; tile += pairs, ++n) {
       const int b = n & 1;
       int tt, ft;
       tile_at(p, tile, tt, ft);
       const int t0 = tt * kTileM + rank * kRowsM + q * 32, f0 = ft * tile_f;
-      const float xs = next_x;
+      float xs = next_x;
       __syncwarp();
 #pragma unroll
       for (int k = 0; k < PER_LANE; ++k) {
@@ -566,7 +585,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       }
       __syncwarp();
       if (tile + pairs < tiles) fetch(tile + pairs);
-      if (!warp_agrees(mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc, p.wait_ns))) break;
+      // after a wait that ran out, this and the tiles that follow are NaN, not the memory's old values
+      ok = ok && warp_agrees(mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc, p.wait_ns));
+      if (!ok) xs = __uint_as_float(0x7fc00000u);
       tc_fence_after();
       const uint32_t from = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kTileN;
       for (int c = half * CH, i0 = 0; c < tile_f; c += 2 * CH, i0 += CH) {

@@ -113,6 +113,11 @@ __device__ __forceinline__ bool mbar_wait_drain(uint32_t bar, uint32_t parity) {
     if ((i & 63u) == 0u && globaltimer() - t0 > kDrainBudgetNs) return false;
   }
 }
+// The same for copies whose barrier this thread cannot wait on: the limit itself.
+__device__ __forceinline__ void pause_drain() {
+  const uint64_t t0 = globaltimer();
+  while (globaltimer() - t0 < kDrainBudgetNs) {}
+}
 
 // ---- L2 cache policies ----------------------------------------------------
 __device__ __forceinline__ uint64_t policy_evict_first() {

@@ -104,7 +104,8 @@ def int8_ffn(x: torch.Tensor, x_scale: torch.Tensor, w13: torch.Tensor, w13_scal
 
 def int8_check(device: Optional[torch.device] = None) -> None:
     """Synchronize and raise (DeviceTimeoutError) if a bounded device wait of
-    ``int8_linear`` or ``int8_ffn`` gave up on this device (default: the current one)."""
+    ``int8_linear`` or ``int8_ffn`` gave up on this device (default: the current one) since
+    the last call. What such a call could not finish is NaN."""
     with torch.cuda.device(device):
         check(lib().mm_int8_check(), "int8_check")
 

@@ -67,3 +67,35 @@ def test_a_wait_of_the_block_runs_out():
             megamoe.int8_check()
         assert torch.equal(megamoe.int8_ffn(x, xs, w13, s13, w2, s2), want)
         megamoe.int8_check()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("tokens,features,depth,ranks", FORMS)
+def test_what_a_failed_launch_could_not_finish_is_nan(tokens, features, depth, ranks, dtype):
+    """No value of a launch whose wait ran out looks valid without being right: the CTAs that
+    share a tile's depth all know of it, and what none of them could finish is NaN."""
+    call = operands(tokens, features, depth)
+    want = megamoe.int8_linear(*call, out_dtype=dtype)
+    for rank in ranks:
+        got = torch.full_like(want, 7.0)
+        _lib.lib().mm_int8_withhold(rank, 1)
+        megamoe.int8_linear(*call, out_dtype=dtype, out=got)
+        with pytest.raises(_lib.DeviceTimeoutError):
+            megamoe.int8_check()
+        assert bool(got.isnan().any())
+        assert bool((got.isnan() | (got == want)).all()), int((~(got.isnan() | (got == want))).sum())
+
+
+@pytest.mark.parametrize("tokens", [3, 20, 100, 600])
+def test_a_failed_product_of_the_block_reaches_its_rows(tokens):
+    """The gated product's rows are a workspace: what it could not finish is not taken from the
+    call before."""
+    x, xs, w13, s13 = operands(tokens, 1024, 2048)
+    _, _, w2, s2 = operands(1, 2048, 512)
+    want = megamoe.int8_ffn(x, xs, w13, s13, w2, s2)
+    megamoe.int8_ffn(x.flip(0).contiguous(), xs * 0.5, w13, s13, w2, s2)
+    _lib.lib().mm_int8_withhold(0, 1)
+    got = megamoe.int8_ffn(x, xs, w13, s13, w2, s2)
+    with pytest.raises(_lib.DeviceTimeoutError):
+        megamoe.int8_check()
+    assert bool(got.isnan().any()) and bool((got.isnan() | (got == want)).all())
