@@ -72,6 +72,31 @@ struct alignas(64) Int8Args {
   uint64_t wait_ns;     // budget of every bounded wait (mm_int8_set_wait_budget)
 };
 
+// A bounded wait for the phase of `bar` with this parity (CLUSTER: other CTAs arrive on it too).
+// One that runs out sets the error word, for the host alone, and `failed`, this CTA's own, at which
+// the CTA's other waits give up; no other launch's waits do.
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile uint32_t *failed, uint32_t code, uint64_t budget_ns) {
+  auto there = [&] { return CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity); };
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (there()) return true;
+  const uint64_t t0 = globaltimer();
+#pragma unroll 1
+  for (uint32_t i = 0;; ++i) {
+    if (there()) return true;
+    if ((i & 63u) == 0u) {
+      if (*failed) return false;
+      if (globaltimer() - t0 > budget_ns) {
+        error_raise(&g_int8_error, code);
+        *failed = 1u;
+        __threadfence_block();
+        return false;
+      }
+    }
+  }
+}
+
 // A whole warp waits, one elected lane issues: the lanes go on together, or give up together.
 __device__ __forceinline__ bool warp_agrees(bool ok) { return __all_sync(0xffffffffu, ok); }
 
@@ -221,7 +246,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
     for (; i < loads; ++i) {
       const int s = i % S::kStages;
       if (i >= S::kStages &&
-          !warp_agrees(mbar_wait(empty + 8 * s, ((i / S::kStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty, p.wait_ns)))
+          !warp_agrees(wait_for<false>(empty + 8 * s, ((i / S::kStages) - 1) & 1, failed, kErrTimeoutEmpty, p.wait_ns)))
         break;
       if (elect_one()) {
         if (i >= early) load_w(i);
@@ -236,11 +261,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
     constexpr uint32_t idesc = idesc_i8(kRowsM, BN);
     for (int i = 0; i < n; ++i) {
       const int s = i % S::kStages;
-      if (!warp_agrees(mbar_wait(full + 8 * s, (i / S::kStages) & 1, &g_int8_error, kErrTimeoutFull, p.wait_ns))) {
-        *failed = 1u;
-        __threadfence_block();
-        break;
-      }
+      if (!warp_agrees(wait_for<false>(full + 8 * s, (i / S::kStages) & 1, failed, kErrTimeoutFull, p.wait_ns))) break;
       tc_fence_after();
       const uint32_t stage = ring + s * S::kStageBytes;
       const uint64_t w = smem_desc(stage, 16, 1024, kLayoutSw128);
@@ -272,7 +293,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
     second[i] = i >= left ? 0.0f : GATED ? p.w_scale[static_cast<int64_t>(p.features) + f + i] : p.bias ? p.bias[f + i] : 0.0f;
   }
   if (warp >= 2 && threadIdx.x - 64 < live) x_scale[threadIdx.x - 64] = p.x_scale[t0 + threadIdx.x - 64];
-  const bool ok = warp_agrees(mbar_wait(acc, 0, &g_int8_error, kErrTimeoutAcc, p.wait_ns) && *failed == 0u);
+  const bool ok = warp_agrees(wait_for<false>(acc, 0, failed, kErrTimeoutAcc, p.wait_ns) && *failed == 0u);
   if (!ok) pause_drain();  // copies still in flight land before this CTA's marks below, not over them
   tc_fence_after();
   // Every CTA of the cluster finishes the tokens rank, rank + split, ... Groups of four warps read the
@@ -333,7 +354,7 @@ __global__ void __launch_bounds__(Stream<BN, GATED>::kWarps * 32) int8_stream_ke
     __syncthreads();  // x's scales, and the TMEM reads
     if (warp == 1) tmem_dealloc(tmem, S::kCols);
     if (rank >= live) return;
-    const bool came = warp_agrees(mbar_wait_cluster(recv, 0, &g_int8_error, kErrTimeoutAcc, p.wait_ns));
+    const bool came = warp_agrees(wait_for<true>(recv, 0, failed, kErrTimeoutAcc, p.wait_ns));
 #pragma unroll 1
     for (int j = rank + split * warp; j < live; j += split * S::kWarps) {
       const int *part = reinterpret_cast<const int *>(ring_ptr) + (j & ~(split - 1)) * kRowsM + PER * lane;
@@ -430,6 +451,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
   const uint32_t full = bars, empty = full + 8 * kTileStages, acc_full = empty + 8 * kTileStages,
                  acc_empty = acc_full + 16, drained = acc_empty + 16, slot = drained + 8;
   uint32_t *slot_ptr = reinterpret_cast<uint32_t *>(base + (slot - ring));
+  volatile uint32_t *failed = slot_ptr + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = static_cast<int>(cluster_rank());
@@ -451,6 +473,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       mbar_init(acc_empty + 8 * b, 2 * kEpilogueWarps);  // of both CTAs
     }
     mbar_init(drained, 1);
+    *failed = 0u;
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -481,7 +504,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
         }
         const int s = it % kTileStages;
         if (it >= kTileStages &&
-            !warp_agrees(mbar_wait_cluster(empty + 8 * s, ((it / kTileStages) - 1) & 1, &g_int8_error, kErrTimeoutEmpty, p.wait_ns))) {
+            !warp_agrees(wait_for<true>(empty + 8 * s, ((it / kTileStages) - 1) & 1, failed, kErrTimeoutEmpty, p.wait_ns))) {
           ok = false;
           break;
         }
@@ -516,11 +539,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       bool ok = true;
       for (int tile = pair; tile < tiles && ok; tile += pairs, ++n) {
         const int b = n & 1;
-        if (n >= 2 && !warp_agrees(mbar_wait_cluster(acc_empty + 8 * b, ((n >> 1) - 1) & 1, &g_int8_error, kErrTimeoutAcc, p.wait_ns))) break;
+        if (n >= 2 && !warp_agrees(wait_for<true>(acc_empty + 8 * b, ((n >> 1) - 1) & 1, failed, kErrTimeoutAcc, p.wait_ns))) break;
         tc_fence_after();
         for (int kb = 0; kb < p.blocks_k; kb += kTileBlocks, ++it) {
           const int s = it % kTileStages;
-          if (!warp_agrees(mbar_wait_cluster(full + 8 * s, (it / kTileStages) & 1, &g_int8_error, kErrTimeoutFull, p.wait_ns))) {
+          if (!warp_agrees(wait_for<true>(full + 8 * s, (it / kTileStages) & 1, failed, kErrTimeoutFull, p.wait_ns))) {
             ok = false;
             break;
           }
@@ -586,7 +609,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       __syncwarp();
       if (tile + pairs < tiles) fetch(tile + pairs);
       // after a wait that ran out, this and the tiles that follow are NaN, not the memory's old values
-      ok = ok && warp_agrees(mbar_wait_cluster(acc_full + 8 * b, (n >> 1) & 1, &g_int8_error, kErrTimeoutAcc, p.wait_ns));
+      ok = ok && warp_agrees(wait_for<true>(acc_full + 8 * b, (n >> 1) & 1, failed, kErrTimeoutAcc, p.wait_ns));
       if (!ok) xs = __uint_as_float(0x7fc00000u);
       tc_fence_after();
       const uint32_t from = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kTileN;

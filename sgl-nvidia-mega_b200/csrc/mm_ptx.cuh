@@ -399,7 +399,7 @@ __device__ __forceinline__ void tc_pair_mma_i8(uint32_t d_tmem, uint64_t adesc, 
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// mbar_wait on a barrier that the other CTA of the pair arrives on too.
+// mbar_try_wait on a barrier that other CTAs of the cluster arrive on too.
 __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -410,24 +410,6 @@ __device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t par
       : "r"(bar), "r"(parity)
       : "memory");
   return ok != 0u;
-}
-__device__ __forceinline__ bool mbar_wait_cluster(uint32_t bar, uint32_t parity, uint32_t *err, uint32_t code,
-                                                  uint64_t budget_ns = kWaitBudgetNs) {
-#pragma unroll 1
-  for (int i = 0; i < 256; ++i)
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-  const uint64_t t0 = globaltimer();
-#pragma unroll 1
-  for (uint32_t i = 0;; ++i) {
-    if (mbar_try_wait_cluster(bar, parity)) return true;
-    if ((i & 63u) == 0u) {
-      if (error_set(err)) return false;
-      if (globaltimer() - t0 > budget_ns) {
-        error_raise(err, code);
-        return false;
-      }
-    }
-  }
 }
 // Arrive on `bar` of both CTAs of the pair once every MMA this thread issued has completed.
 __device__ __forceinline__ void tc_pair_commit(uint32_t bar) {

@@ -99,3 +99,27 @@ def test_a_failed_product_of_the_block_reaches_its_rows(tokens):
     with pytest.raises(_lib.DeviceTimeoutError):
         megamoe.int8_check()
     assert bool(got.isnan().any()) and bool((got.isnan() | (got == want)).all())
+
+
+@pytest.mark.parametrize("tokens,features,depth", [(4, 300, 7168), (100, 300, 7168), (600, 1000, 2048)])
+def test_a_launch_keeps_its_budget_after_another_failed(tokens, features, depth):
+    """The word that int8_check reads belongs to the device: a wait that ran out in one launch,
+    unread, is no reason for another launch's waits to give up."""
+    call = operands(tokens, features, depth)
+    want = megamoe.int8_linear(*call)
+    _lib.lib().mm_int8_withhold(0, 1)
+    megamoe.int8_linear(*operands(4, 300, 7168))
+    torch.cuda.synchronize()
+    megamoe.int8_set_wait_budget(400_000)
+    _lib.lib().mm_int8_withhold(0, 1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    t0 = time.perf_counter()
+    with torch.cuda.stream(side):
+        megamoe.int8_linear(*call)
+    torch.cuda.synchronize()
+    assert 0.4 <= time.perf_counter() - t0 < 2.0
+    assert torch.equal(megamoe.int8_linear(*call), want)
+    with pytest.raises(_lib.DeviceTimeoutError):
+        megamoe.int8_check()
+    megamoe.int8_check()
