@@ -24,8 +24,8 @@ struct NormArgs {
   int gamma_f32;             // gamma is fp32 beside a 16-bit x
   int gamma_wide;            // gamma starts on a 16-byte boundary
   int codes_wide;            // code rows start on 8-byte boundaries
-  int turn_bytes;            // shared memory of a row of them
   int code_row;              // int8 codes on 16-byte boundaries of rows that are not
+  int turn_bytes;            // shared memory in which a row of such codes is turned
 };
 
 // The code rint(y / s), in the low byte. y / s by y * r, r = 1 / s, and one correction from the

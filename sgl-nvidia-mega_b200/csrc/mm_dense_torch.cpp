@@ -1,7 +1,7 @@
 // The dense 8-bit operators' calls on torch tensors: checks, outputs and workspace from
 // torch's allocator, the tensors' device and its current stream, then one call of the C ABI
 // (include/megamoe.h). Python's share of such a call (attribute lookups, ctypes, four
-// torch.empty) took 12 to 21 us, several times the kernel of a decode step; here it is a few.
+// torch.empty) took 14 to 24 us, several times the kernel of a decode step; here it is 4 to 9.
 // megamoe/dense.py holds the documented functions.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>

@@ -727,6 +727,12 @@ int rounds(int tokens, int warps, int regs) {
 // of 8192 x 2048: two 25.6, four 26.0), rows between by the rounds (norm of 640 x 6147: two 7.3, four
 // 8.3; of 1024 x 6147: two 9.9, four 9.0). int8 rows alone hold less beside the row: 4096 x 16384: four
 // 42, eight 35; 8192 x 7168: two 41, four 33, eight 30.5.
+// The norm's rows of more than 512 chunks: two chunks a thread against four, as two's time over four's in a
+// sweep of 450..8192 rows (bf16 of 4608..8192 values, fp32 of 2304..4096). Up to 832 chunks and 2048 rows either
+// may win (norm alone 0.82..1.31, with MXFP8 0.77..1.22, with int8 0.74..1.15), and fewer rounds tell which; more
+// rows 0.94..1.38, longer rows 0.81..1.64: four. The rule takes the better one or is within 4 % of it at 256 of the 280
+// sizes, within 11 % at all of bf16's; what it misses most is fp32 with MXFP8 or without codes from 833 chunks
+// on at 450..1536 rows (600 x 4096 with MXFP8: four 9.4 us, two 7.6).
 template <typename T, int QUANT, bool NORM, bool TURN>
 cudaError_t launch_rows(NormArgs a, int chunks, void *stream) {
   constexpr bool kDense = QUANT == MM_QUANT_NONE && sizeof(T) == 2;
@@ -735,8 +741,9 @@ cudaError_t launch_rows(NormArgs a, int chunks, void *stream) {
   constexpr auto four = norm_rows_kernel<T, 4, QUANT, NORM, TURN, false>;
   constexpr auto eight = norm_rows_kernel<T, 8, QUANT, NORM, TURN, false>;
   a.turn_bytes = TURN ? static_cast<int>((chunks * (16 / sizeof(T)) + 32) / 16 * 16 + 16) : 0;
-  // Short rows in number share CTAs, a warp each (int8 rows of 8192 x 1024 5.4 us instead of 9.2,
-  // norm of 8192 x 512 6.1 instead of 9.4; norm with int8 of 1300 x 1024 6.0 instead of 4.4).
+  // Short rows share CTAs, a warp each, from kShareRows rows on (int8 rows of 8192 x 1024: shared 5.4 us,
+  // a CTA each 9.2; norm of 8192 x 512: 6.1 and 9.4). Fewer rows lose by it (norm with int8 of 1300 x
+  // 1024: shared 6.0, a CTA each 4.4).
   const int share = chunks > 128 || a.tokens < kShareRows ? 1 : a.tokens < 2 * kShareRows ? 4 : 8;
   const bool dense = kDense && share == 1 && chunks <= 4 * row_threads(4, NORM, true);
   auto warps = [&](int n) { return (chunks + 32 * n - 1) / (32 * n); };

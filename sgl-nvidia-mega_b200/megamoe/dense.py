@@ -12,7 +12,9 @@
 
 Every call runs on the current stream of the tensors' device, allocates its
 outputs and its workspace from torch's allocator (so calls on several streams,
-and captured graphs, share none) and never synchronizes. Tensors are 2-D with
+and captured graphs, share none) and never synchronizes. What calls share is one
+word a device, set when a bounded wait of an int8 product runs out and read by
+``int8_check``. Tensors are 2-D with
 their last dimension contiguous; rows may be strided. An output given as ``out=``
 may not share memory with an input (``rms_norm``'s ``residual_out`` may; columns beside
 each other of one buffer's rows share none). Outputs of
@@ -82,9 +84,10 @@ def quantize_int8(x: torch.Tensor):
 def int8_linear(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
                 bias: Optional[torch.Tensor] = None, *, out_dtype: torch.dtype = torch.bfloat16,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """out[t, n] = (sum_k x[t, k] weight[n, k]) * x_scale[t] * weight_scale[n] + bias[n],
-    one rounding to ``out_dtype`` (bf16, fp16 or fp32) from an exact integer sum:
-    x int8 [T, K] (``rms_norm`` / ``quantize_int8`` codes), weight int8 [N, K], both with
+    """out[t, n] = (sum_k x[t, k] weight[n, k]) * x_scale[t] * weight_scale[n] + bias[n]:
+    the sum is an exact integer, its conversion, the product with x_scale and the last
+    product with the bias (fused) round in fp32, and the result to ``out_dtype`` (bf16,
+    fp16 or fp32). x int8 [T, K] (``rms_norm`` / ``quantize_int8`` codes), weight int8 [N, K], both with
     rows on 16-byte boundaries, scales fp32 [T] and [N] (or [.., 1]), bias fp32 [N].
     K < 131072."""
     return (_dense or _load()).int8_linear(x, x_scale, weight, weight_scale, bias, out_dtype, out)
