@@ -524,13 +524,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTileThreads, 1) int
       }
     }
     // leave no copy in flight: the last stages' barriers complete with both CTAs' copies
-    if (rank == 0) {
+    if (rank == 0)
       for (int j = max(0, it - kTileStages); j < it; ++j)
         mbar_wait_drain(full + 8 * (j % kTileStages), (j / kTileStages) & 1);
-    } else if (!ok) {
-      // the leader may have stopped before this CTA did, and then has not waited for all of its copies
-      pause_drain();
-    }
+    // where either CTA stopped early, the other's later copies are on no barrier that completes
+    if (!ok) pause_drain();
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0) {
